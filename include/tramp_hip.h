@@ -558,6 +558,49 @@ int tramp_conv_message(tramp_ctx* ctx, tramp_conv* conv, int dir, size_t batch,
                        double damping, const double* a_old_d, const void* b_old_d,
                        double* a_new_d, void* b_new_d, void* r_d, double* v_d, int reuse);
 
+/* ---- lookup channel x_t = scale z[token_t] ---------------------------------------- */
+/* The linear channel of categorical data: the design matrix W of LinearChannel (tramp/channels/linear/linear_channel.py:18-132)
+ * with one entry `scale` per row, for z = [batch, n_rows, n_cols] and x = [batch, n_pos, n_cols].  tokens_h (host): [n_pos],
+ * the row each position reads, -1 for a padded position (a zero row of W: x = 0 there).  The positions are sorted by token
+ * once, here; W^T W = scale^2 diag(count) makes variances, messages and log-partition closed forms (csrc/lookup.hip).
+ * n_rows, n_cols, n_pos < 2^31 - 1; sums over positions are in double, in a fixed order, without atomics. */
+typedef struct tramp_lookup tramp_lookup;
+int tramp_lookup_create(tramp_ctx* ctx, int dtype, size_t n_rows, size_t n_cols, size_t n_pos, const int* tokens_h,
+                        double scale, tramp_lookup** lookup);
+int tramp_lookup_destroy(tramp_ctx* ctx, tramp_lookup* lookup);
+/* x[b, t, :] = scale z[b, token_t, :] (0 where padded). */
+int tramp_lookup_apply(tramp_ctx* ctx, tramp_lookup* lookup, size_t batch, const void* z_d, void* x_d);
+/* The adjoint: g[b, v, :] = scale sum of x[b, t, :] over the positions t of token v (0 for a token without positions). */
+int tramp_lookup_gradient(tramp_ctx* ctx, tramp_lookup* lookup, size_t batch, const void* x_d, void* g_d);
+/* LinearChannel.compute_n_eff / compute_*_variance (linear_channel.py:58-67, 91-105); v_d, a_new_d, n_eff_d optional. */
+int tramp_lookup_variance(tramp_ctx* ctx, tramp_lookup* lookup, int dir, size_t batch, const double* az_d, const double* ax_d,
+                          double* v_d, double* a_new_d, double* n_eff_d);
+/* dir BWD: the message to z ([batch, n_rows, n_cols]), FWD: to x ([batch, n_pos, n_cols]); r_d, v_d optional posterior.
+ * b_new_d must not be bz_d or bx_d; a_old_d / b_old_d may be the outputs. */
+int tramp_lookup_message(tramp_ctx* ctx, tramp_lookup* lookup, int dir, size_t batch, const double* az_d, const void* bz_d,
+                         const double* ax_d, const void* bx_d, double damping, const double* a_old_d, const void* b_old_d,
+                         double* a_new_d, void* b_new_d, void* r_d, double* v_d);
+int tramp_lookup_log_partition(tramp_ctx* ctx, tramp_lookup* lookup, size_t batch, const double* az_d, const void* bz_d,
+                               const double* ax_d, const void* bx_d, double* out_d);
+
+/* ---- lists of arrays: global norm, clipping, bounded steps -------------------------- */
+/* k arrays [batch, n_i] of one element type; row b of all of them is instance b, whose global norm is
+ * |x_b| = sqrt(sum over the arrays and components of x^2), summed in double in a fixed order.  arrays_d: host array of device
+ * pointers, kept as they are (the caller keeps the arrays alive and in place); the arrays must not overlap. */
+typedef struct tramp_group tramp_group;
+int tramp_group_create(tramp_ctx* ctx, int dtype, int k, void* const* arrays_d, const size_t* n, size_t batch, tramp_group** group);
+int tramp_group_destroy(tramp_ctx* ctx, tramp_group* group);
+int tramp_group_norm(tramp_ctx* ctx, const tramp_group* group, double* norm_d);
+/* out = x min(1, max_norm / |x_b|); out is `group` itself (in place) or arrays clear of it; norm_d [batch] (optional): |x_b|
+ * before.  An instance whose norm is not finite is copied as it is. */
+int tramp_group_clip(tramp_ctx* ctx, const tramp_group* group, double max_norm, const tramp_group* out, double* norm_d);
+/* out = prev + min(1, max_step / |x_b - prev_b|) (x - prev), the step of a set of messages bounded like constant damping with a
+ * factor per instance (tramp/algos/message_passing.py:119-127).  a_d, a_prev_d [n_a, batch] (optional): precisions that move
+ * by the same factor, in place in a_d.  refresh != 0: the result is written over prev (and a_prev) as well.  An instance whose
+ * step is not finite takes it whole, for the NaN guard to see. */
+int tramp_group_limit_step(tramp_ctx* ctx, const tramp_group* group, const tramp_group* prev, double max_step,
+                           const tramp_group* out, int refresh, size_t n_a, double* a_d, double* a_prev_d, double* norm_d);
+
 /* ---- gradient channel x = grad z --------------------- */
 /* GradientChannel (tramp/channels/linear/gradient_channel.py:10-118, real=True): one circular
  * forward-difference filter per axis (d = ndim), x = [batch, d, n] for z = [batch, n]; diagonal in

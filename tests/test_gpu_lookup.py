@@ -1,0 +1,388 @@
+"""GPU: the lookup channel against its definitions in 64 bits.
+
+Tolerances count roundings.  The kernels compute in double (u = 2^-53) and round once to the element type (half a step,
+eps / 2).  A sum of c terms is off by at most (c - 1) u times the sum of their magnitudes on either side, a quotient, product
+or sum by u each; the precision a' of a message is a ratio of sums of K positive terms of at most 8 operations, so it is off
+by at most 2 (K + 8) u relative, in the kernel; the definition takes it in rational numbers and rounds once.  The bounds
+below take 2 (c + 2 K + 32) u of the sum of magnitudes of every term of a formula: both sides' share."""
+import ctypes as C
+
+import numpy as np
+import pytest
+
+from oracle import tramp_oracle as orc
+from tests.lookup_plain import LookupFactor, dense_of, zipf_tokens
+
+pytestmark = pytest.mark.gpu
+U = 2.0**-53
+
+# V, positions, D, zipf exponent, padded share
+SHAPES = [(1, 1, 1, 0.0, 0.0), (1, 5, 3, 0.0, 0.0), (7, 1, 1, 0.0, 0.0), (50, 200, 1, 1.0, 0.1), (33, 257, 5, 1.0, 0.2),
+          (64, 1000, 64, 1.0, 0.0), (10, 5000, 16, 0.5, 0.05), (1000, 10, 4, 0.0, 0.0), (3, 20011, 2, 0.3, 0.0),
+          (1, 70001, 1, 0.0, 0.5), (300, 900, 260, 1.2, 0.0), (40, 300, 1030, 1.0, 0.3), (4099, 30011, 1, 1.1, 0.0),
+          (20, 4, 8, 0.0, 1.0), (513, 2048, 12, 0.8, 0.0), (2, 9000, 130, 0.0, 0.0)]
+
+
+def make(T, ctx, shape, dtype, batch, scale, seed=0):
+    V, n, D, z, pad = shape
+    rs = np.random.RandomState(seed + V + 7 * n + 13 * D)
+    tok = zipf_tokens(rs, V, n, z, pad)
+    ch = T.LookupChannel(tok, V, dim=D, scale=scale, padding_index=-1, dtype=dtype, ctx=ctx)
+    draw = lambda m: rs.standard_normal((batch, m)).astype(dtype)            # noqa: E731
+    return ch, LookupFactor(tok, V, D, scale), rs, draw(V * D), draw(n * D)
+
+
+def eps2(dtype):
+    return np.finfo(dtype).eps / 2
+
+
+@pytest.mark.parametrize("dtype", [np.float64, np.float32])
+@pytest.mark.parametrize("shape", SHAPES, ids=lambda s: "x".join(map(str, s[:3])))
+def test_lookup_and_gradient(ctx, shape, dtype):
+    import tramp_amd as T
+    for batch, scale in ((1, 1.0), (3, -1.7)):
+        ch, ref, rs, z, x = make(T, ctx, shape, dtype, batch, scale)
+        zd, xd = ctx.array(z, dtype), ctx.array(x, dtype)
+        X, G = ch.lookup(zd).get(), ch.gradient(xd).get()
+        cmax = ref.count.max()
+        for b in range(batch):
+            want = ref.lookup(z[b]).reshape(-1)
+            assert np.array_equal(X[b] == 0, want == 0)
+            assert (np.abs(X[b] - want) <= (eps2(dtype) + 2 * U) * np.abs(want)).all()
+            want = ref.gradient(x[b]).reshape(-1)
+            mag = np.abs(scale) * LookupFactor(ref.tok, ref.V, ref.D, 1.0).gradient(np.abs(x[b])).reshape(-1)
+            assert (np.abs(G[b] - want) <= eps2(dtype) * np.abs(want) + 2 * (cmax + 2) * U * mag).all()
+        # the adjoint identity <lookup z, x> = <z, gradient x> and, the map being linear, its difference quotient
+        left, right = np.sum(X.astype(float) * x), np.sum(z.astype(float) * G)
+        size = np.sum(np.abs(X.astype(float) * x)) + np.sum(np.abs(z.astype(float) * G))
+        assert abs(left - right) <= (2 * eps2(dtype) + (cmax + x.size + z.size + 8) * U) * size + 1e-300
+        dz = rs.standard_normal(z.shape).astype(dtype)
+        z2 = (z.astype(float) + dz).astype(dtype)
+        diff = ch.lookup(ctx.array(z2, dtype)).get().astype(float) - X
+        want = np.stack([ref.lookup(z2[b].astype(float) - z[b]).reshape(-1) for b in range(batch)])
+        lim = (eps2(dtype) + 4 * U) * abs(scale) * np.stack([LookupFactor(ref.tok, ref.V, ref.D, 1.0).lookup(np.abs(z2[b]).astype(float) + np.abs(z[b])).reshape(-1)
+                                                         for b in range(batch)])
+        assert (np.abs(diff - want) <= lim).all()
+
+
+def magnitudes(ref, az, bz, ax, bx, a, direction):
+    "sum of the magnitudes of the terms of b'"
+    lik, prec = (ax * ref.s**2 * ref.count)[:, None], ref._prec(az, ax)[:, None]
+    g = abs(ref.s) * LookupFactor(ref.tok, ref.V, ref.D, 1.0).gradient(np.abs(bx.astype(float)))
+    zz = np.abs(bz.astype(float)).reshape(ref.V, ref.D)
+    if direction == "backward":
+        return ((g * (az + a) + zz * (a + lik)) / prec).reshape(-1)
+    r = np.zeros((ref.T, ref.D))
+    r[ref.at] = abs(ref.s) * ((zz + g) / prec)[ref.tok[ref.at]]
+    return r.reshape(-1) * (ax + a) + np.abs(bx.astype(float))
+
+
+@pytest.mark.parametrize("dtype", [np.float64, np.float32])
+@pytest.mark.parametrize("direction", ["forward", "backward"])
+@pytest.mark.parametrize("shape", SHAPES, ids=lambda s: "x".join(map(str, s[:3])))
+def test_messages(ctx, shape, direction, dtype):
+    import tramp_amd as T
+    batch, scale = 4, 1.3
+    ch, ref, rs, z, x = make(T, ctx, shape, dtype, batch, scale)
+    az, ax = np.array([0.7, 1e-3, 2.0, 40.0]), np.array([1.9, 3e2, 0.0, 1e-4])
+    n = x.shape[1] if direction == "forward" else z.shape[1]
+    message = getattr(ch, f"compute_{direction}_message")
+    posterior = getattr(ch, f"compute_{direction}_posterior")
+    a_d, b_d = message(ctx.scalars(az), ctx.array(z, dtype), ctx.scalars(ax), ctx.array(x, dtype))
+    r_d, v_d = posterior(ctx.scalars(az), ctx.array(z, dtype), ctx.scalars(ax), ctx.array(x, dtype))
+    a0, b0 = rs.uniform(0.1, 2.0, batch), rs.standard_normal((batch, n)).astype(dtype)
+    old_a, old_b = ctx.scalars(a0), ctx.array(b0, dtype)
+    message(ctx.scalars(az), ctx.array(z, dtype), ctx.scalars(ax), ctx.array(x, dtype), out_a=old_a, out_b=old_b, damping=0.3,
+            old_a=old_a, old_b=old_b)                                        # in place
+    A, B, R, Vv, DA, DB = a_d.get(), b_d.get(), r_d.get(), v_d.get(), old_a.get(), old_b.get()
+    K = np.unique(ref.count).size
+    for i in range(batch):
+        ra, rb = getattr(ref, direction)(az[i], z[i], ax[i], x[i])
+        rel_a = 2 * (K + 8) * U
+        assert abs(A[i] - ra) <= 2 * rel_a * ra + 1e-300, (i, A[i], ra)
+        k = 2 * (ref.count.max() + 2 * K + 32) * U
+        mag = magnitudes(ref, az[i], z[i], ax[i], x[i], ra, direction)
+        assert (np.abs(B[i] - rb) <= eps2(dtype) * np.abs(rb) + k * mag).all(), i
+        assert abs(DA[i] - (0.3 * a0[i] + 0.7 * ra)) <= 2 * rel_a * (a0[i] + ra)
+        want = 0.3 * b0[i].astype(float) + 0.7 * rb
+        assert (np.abs(DB[i] - want) <= eps2(dtype) * np.abs(want) + k * (mag + np.abs(b0[i]))).all()
+        mean = ref.mean(az[i], z[i], ax[i], x[i])
+        if direction == "forward":
+            mean = np.where(ref.tok[:, None] >= 0, ref.s * mean[np.maximum(ref.tok, 0)], 0.0)
+        lim = k * mag / ((ax[i] if direction == "forward" else az[i]) + ra)   # mag holds |r| (a + a')
+        assert (np.abs(R[i] - mean.reshape(-1)) <= eps2(dtype) * np.abs(mean.reshape(-1)) + lim).all()
+        v = float(getattr(ref, direction + "_variance")(az[i], ax[i]))
+        assert abs(Vv[i] - v) <= rel_a * v
+        assert getattr(ch, f"compute_{direction}_variance")(az[i], ax[i]) == pytest.approx(v, rel=rel_a)
+        assert ch.compute_n_eff(az[i], ax[i]) == pytest.approx(ref.n_eff(az[i], ax[i]), rel=2 * rel_a, abs=0)
+
+
+@pytest.mark.parametrize("dtype", [np.float64, np.float32])
+def test_log_partition_and_its_gradient(ctx, dtype):
+    "A of LinearChannel; dA/dbz is the posterior mean: a central difference of a quadratic is exact up to rounding"
+    import tramp_amd as T
+    for shape in SHAPES:
+        if shape[0] * shape[2] > 5000:
+            continue
+        ch, ref, rs, z, x = make(T, ctx, shape, dtype, 2, 0.8)
+        az, ax = np.array([0.7, 3.0]), np.array([1.9, 0.0])
+        A = ch.compute_log_partition(ctx.scalars(az), ctx.array(z, dtype), ctx.scalars(ax), ctx.array(x, dtype)).ravel()
+        for i in range(2):
+            want = ref.log_partition(az[i], z[i], ax[i], x[i])
+            h = np.abs(z[i].astype(float)).reshape(ref.V, ref.D) + 0.8 * LookupFactor(ref.tok, ref.V, ref.D, 1.0).gradient(np.abs(x[i]).astype(float))
+            prec = ref._prec(az[i], ax[i])
+            mag = 0.5 * np.sum(h**2 / prec[:, None]) + 0.5 * ref.D * np.sum(np.abs(np.log(2 * np.pi / prec)) + 2)
+            assert abs(A[i] - want) <= 2 * (z.shape[1] + 2 * ref.count.max() + 16) * U * mag
+        step = np.zeros_like(z)
+        at = rs.randint(z.shape[1])
+        step[:, at] = 0.25
+        up = ch.compute_log_partition(ctx.scalars(az), ctx.array(z + step, dtype), ctx.scalars(ax), ctx.array(x, dtype)).ravel()
+        dn = ch.compute_log_partition(ctx.scalars(az), ctx.array(z - step, dtype), ctx.scalars(ax), ctx.array(x, dtype)).ravel()
+        span = (z + step).astype(float)[:, at] - (z - step)[:, at]            # as the element type holds them
+        for i in range(2):
+            r = ref.mean(az[i], z[i], ax[i], x[i]).reshape(-1)[at]
+            # (A(b + s) - A(b - s')) / (s + s') = r + (s - s') / (2 prec): s = s' up to the element type's rounding
+            slack = 4 * (z.shape[1] + 2 * ref.count.max() + 16) * U * (mag + 1) / 0.5 + 4 * eps2(dtype) * (abs(z[i, at]) + 0.25) / ref._prec(az[i], ax[i]).min()
+            assert abs((up[i] - dn[i]) / span[i] - r) <= slack
+
+
+def test_host_arrays_shapes_and_extremes(ctx):
+    import tramp_amd as T
+    rs = np.random.RandomState(5)
+    tok = np.array([[3, 0, 9], [1, 9, 3]], dtype=np.int64)
+    ch = T.LookupChannel(tok, 4, dim=2, scale=2.0, padding_index=9, ctx=ctx)
+    z = rs.standard_normal((4, 2))
+    x = ch.sample(z)
+    assert x.shape == (2, 3, 2) and np.array_equal(x, np.where((tok == 9)[..., None], 0.0, 2.0 * z[np.minimum(tok, 3)]))
+    assert ch.lookup(np.stack([z, -z])).shape == (2, 2, 3, 2)
+    g = ch.gradient(x)
+    assert g.shape == (4, 2) and np.array_equal(g[2], [0, 0])
+    a, b = ch.compute_forward_message(1.0, z, 2.0, x)
+    assert isinstance(a, float) and b.shape == x.shape
+    a, b = ch.compute_backward_message(1.0, z, 2.0, x)
+    assert isinstance(a, float) and b.shape == z.shape
+    assert isinstance(ch.compute_log_partition(1.0, z, 2.0, x), float)
+    assert ch.second_moment(0.5) == 0.5 * 4.0 * 4 / 6
+    for bad in (z[:3], z.T, x, np.zeros(3)):
+        with pytest.raises(ValueError):
+            ch.lookup(bad)
+    with pytest.raises(ValueError):
+        ch.compute_forward_message(1.0, z, 2.0, np.stack([x, x]))
+    flat = T.LookupChannel(tok.ravel(), 4, padding_index=9, ctx=ctx)
+    assert flat.sample(z[:, 0]).shape == (6,)
+    # all positions padded: W = 0; the table's message is flat, the positions' one pins x to zero
+    none = T.LookupChannel(np.full(5, -1), 3, padding_index=-1, ctx=ctx)
+    a, b = none.compute_backward_message(1.5, np.ones(3), 2.0, np.ones(5))
+    assert a == 1e-11 and np.abs(b).max() < 1e-10
+    a, b = none.compute_forward_message(1.5, np.ones(3), 2.0, np.ones(5))
+    assert a == 1e11 and np.array_equal(b, -np.ones(5))
+    # az = 0: rows without positions stay finite in the message to the table (az is floored at 1e-11)
+    one = T.LookupChannel([1, 1], 3, ctx=ctx)
+    a, b = one.compute_backward_message(0.0, np.zeros(3), 2.0, np.ones(2))
+    assert np.isfinite(a) and np.isfinite(b).all()
+    # infinities and NaN: they reach the rows that read them and no others
+    xs = np.array([np.inf, 1.0, np.nan, 2.0])
+    G = T.LookupChannel([0, 1, 2, 1], 4, ctx=ctx).gradient(xs)
+    assert G[0] == np.inf and G[1] == 3.0 and np.isnan(G[2]) and G[3] == 0.0
+    zs = np.array([np.nan, 1.0, np.inf])
+    X = T.LookupChannel([1, 7, 2], 3, padding_index=7, ctx=ctx).lookup(zs)
+    assert X[0] == 1.0 and X[1] == 0.0 and X[2] == np.inf
+    # a NaN at a padded position touches no row
+    G = T.LookupChannel([0, 7], 2, padding_index=7, ctx=ctx).gradient(np.array([1.0, np.nan]))
+    assert np.array_equal(G, [1.0, 0.0])
+
+
+@pytest.mark.parametrize("dtype", [np.float64, np.float32])
+def test_views_that_are_not_aligned(ctx, dtype):
+    "rows of larger arrays with odd lengths: every 4- or 8-byte boundary gives the same bits"
+    import tramp_amd as T
+    rs = np.random.RandomState(3)
+    tok = zipf_tokens(rs, 37, 501, 1.0, 0.1)
+    for D in (1, 3, 8, 64):
+        ch = T.LookupChannel(tok, 37, dim=D, scale=1.5, padding_index=-1, dtype=dtype, ctx=ctx)
+        z, x = rs.standard_normal(37 * D).astype(dtype), rs.standard_normal(501 * D).astype(dtype)
+        want = None
+        for shift in (0, 1, 2, 3):
+            big = lambda v: T.DeviceArray(ctx, v.shape, dtype, ptr=keep[-1].ptr + shift * v.itemsize, owner=False)   # noqa: E731
+            keep, views = [], []
+            for v in (z, x, z, x, z):
+                keep.append(ctx.array(np.concatenate([np.zeros(shift, dtype), v, np.zeros(4, dtype)]), dtype))
+                views.append(big(v))
+            zz, xx, gout, xout, bout = views
+            ch.lookup(zz, out=xout)
+            ch.gradient(xx, out=gout)
+            ch.compute_backward_message(ctx.scalars(0.7), zz, ctx.scalars(1.1), xx, out_b=bout)
+            a, f = ch.compute_forward_message(ctx.scalars(0.7), zz, ctx.scalars(1.1), xx)
+            got = [xout.get(), gout.get(), bout.get(), f.get()]
+            ends = [k.get()[shift + len(v):] for k, v in zip(keep, (z, x, z, x, z))]
+            assert all(np.array_equal(e, np.zeros(4, dtype)) for e in ends)   # nothing written behind
+            if want is None:
+                want = got
+            for u, w in zip(got, want):
+                assert np.array_equal(u, w)
+
+
+def test_many_instances_and_no_instance_mixing(ctx):
+    import tramp_amd as T
+    rs = np.random.RandomState(8)
+    tok = zipf_tokens(rs, 19, 70, 1.0, 0.1)
+    ch = T.LookupChannel(tok, 19, dim=3, padding_index=-1, ctx=ctx)
+    B = 301
+    z, x = rs.standard_normal((B, 57)), rs.standard_normal((B, 210))
+    az, ax = rs.uniform(0.5, 2, B), rs.uniform(0.1, 3, B)
+    a, b = ch.compute_forward_message(ctx.scalars(az), ctx.array(z), ctx.scalars(ax), ctx.array(x))
+    A, Bn = a.get(), b.get()
+    for i in (0, 7, 300):
+        a1, b1 = ch.compute_forward_message(ctx.scalars(az[i]), ctx.array(z[i]), ctx.scalars(ax[i]), ctx.array(x[i]))
+        assert a1.get()[0] == A[i] and np.array_equal(b1.get(), Bn[i])
+
+
+def test_captured_calls_replay_and_share_workspaces(ctx):
+    "two graphs and eager calls between the replays, all on one context: every replay gives the eager bits"
+    import tramp_amd as T
+    rs = np.random.RandomState(11)
+    sets = []
+    for V, n, D, dt in ((50, 20000, 3, np.float64), (400, 3000, 64, np.float32)):
+        tok = zipf_tokens(rs, V, n, 1.0, 0.1)
+        ch = T.LookupChannel(tok, V, dim=D, padding_index=-1, dtype=dt, ctx=ctx)
+        s = dict(ch=ch, z=ctx.array(rs.standard_normal((2, V * D)), dt), x=ctx.array(rs.standard_normal((2, n * D)), dt),
+                 az=ctx.scalars([0.5, 1.0]), ax=ctx.scalars([2.0, 0.3]), oa=ctx.empty((2,)), ob=ctx.empty((2, n * D), dt),
+                 pa=ctx.empty((2,)), pb=ctx.empty((2, V * D), dt))
+
+        def calls(s):
+            s["ch"].compute_forward_message(s["az"], s["z"], s["ax"], s["x"], out_a=s["oa"], out_b=s["ob"])
+            s["ch"].compute_backward_message(s["az"], s["z"], s["ax"], s["x"], out_a=s["pa"], out_b=s["pb"])
+        calls(s)
+        s["want"] = [s[k].get() for k in ("oa", "ob", "pa", "pb")]
+        sets.append(s)
+    for s in sets:
+        ctx._call("tramp_graph_begin")
+        calls(s)
+        s["graph"] = C.c_void_p()
+        ctx._call("tramp_graph_end", C.byref(s["graph"]))
+    try:
+        for rep in range(4):
+            for s in sets:
+                for k in ("oa", "ob", "pa", "pb"):
+                    s[k].fill(-1.0)
+                ctx._call("tramp_graph_launch", s["graph"])
+                got = [s[k].get() for k in ("oa", "ob", "pa", "pb")]
+                assert all(np.array_equal(g, w) for g, w in zip(got, s["want"]))
+                s["ch"].gradient(s["x"])
+            ctx.sync()
+    finally:
+        for s in sets:
+            ctx._call("tramp_graph_destroy", s["graph"])
+
+
+def test_refusals_on_the_device(ctx):
+    import tramp_amd as T
+    ch = T.LookupChannel([0, 1, 1], 2, ctx=ctx)
+    z, x = ctx.array(np.ones(2)), ctx.array(np.ones(3))
+    with pytest.raises(T._lib.TrampHipError):
+        ctx._call("tramp_lookup_apply", ch._handle, 1, z.ptr, z.ptr)
+    with pytest.raises(T._lib.TrampHipError):
+        ctx._call("tramp_lookup_gradient", ch._handle, 1, x.ptr, x.ptr)
+    with pytest.raises(T._lib.TrampHipError):
+        ctx._call("tramp_lookup_apply", ch._handle, 65536, z.ptr, x.ptr)
+    with pytest.raises(ValueError):
+        ch.lookup(z, out=ctx.empty((1, 4)))
+    with pytest.raises(ValueError):
+        ch.lookup(z, out=np.empty(3))
+    with pytest.raises(TypeError):
+        ch.lookup(ctx.array(np.ones(2), np.float32))
+    with pytest.raises(ValueError):
+        ch.gradient(z)
+    a = ctx.scalars(1.0)
+    with pytest.raises(T._lib.TrampHipError):
+        ch.compute_backward_message(a, z, a, x, out_b=z)
+    with pytest.raises(T._lib.TrampHipError):
+        ctx._call("tramp_lookup_message", ch._handle, 0, 1, a.ptr, z.ptr, a.ptr, x.ptr, 0.5, None, None, a.ptr, ctx.empty(3).ptr, None, None)
+    h = C.c_void_p()
+    bad = np.array([0, 5], dtype=np.int32)
+    for args in ((1, 2, 1, 2, bad.ctypes.data, 1.0), (1, 2, 0, 2, bad.ctypes.data, 1.0), (7, 9, 1, 2, bad.ctypes.data, 1.0),
+                 (1, 9, 1, 2, bad.ctypes.data, float("nan")), (1, 9, 1, 2, None, 1.0)):
+        with pytest.raises(T._lib.TrampHipError):
+            ctx._call("tramp_lookup_create", *args, C.byref(h))
+    other = T.Context(0)
+    try:
+        with pytest.raises(ValueError):
+            ch.lookup(other.array(np.ones(2)))
+    finally:
+        other.close()
+
+
+# ---------------------------------------------------------------- in models
+def regression(T, ctx, channel, V, y, prior="gb"):
+    pri = T.GaussBernoulliPrior(size=V, rho=0.5, ctx=ctx)
+    return (pri @ T.SISOVariable(id="x") @ channel @ T.SISOVariable(id="z") @ T.GaussianLikelihood(y=y, var=0.1, ctx=ctx)).to_model()
+
+
+@pytest.mark.parametrize("damping, graph", [(None, False), (0.3, False), (0.3, True)])
+def test_ep_matches_the_dense_channel_and_the_oracle(ctx, damping, graph):
+    import tramp_amd as T
+    rs = np.random.RandomState(2)
+    V, n, B = 60, 150, 3
+    tok = zipf_tokens(rs, V, n, 0.8, 0.1)
+    W = dense_of(tok, V, 1, 1.4)
+    X = np.stack([orc.gb_sample(rs, V, 0.5) for _ in range(B)])
+    Y = X @ W.T + np.sqrt(0.1) * rs.standard_normal((B, n))
+    lk = T.LookupChannel(tok, V, scale=1.4, padding_index=-1, ctx=ctx)
+    ep = T.ExpectationPropagation(regression(T, ctx, lk, V, Y), ctx=ctx)
+    ep.iterate(max_iter=20, callback=T.PassCallback(), damping=damping, graph=graph)
+    r = ep.get_variables_data()["x"]["r"]
+    ref = LookupFactor(tok, V, 1, 1.4)
+    for b in range(B):
+        res = orc.ep_chain([orc.GBPriorFactor(V, rho=0.5), ref, orc.GaussLikFactor(Y[b], 0.1)], [V, n], max_iter=20,
+                           damping=damping, tol=0.0, max_increase=np.inf)
+        assert np.abs(r[b] - res["r"][0]).max() < 1e-9 * np.abs(res["r"][0]).max()
+    dense = T.ExpectationPropagation(regression(T, ctx, T.LinearChannel(W, ctx=ctx, svd="host"), V, Y), ctx=ctx)
+    dense.iterate(max_iter=20, callback=T.PassCallback(), damping=damping)
+    rd = dense.get_variables_data()["x"]["r"]
+    assert np.abs(r - rd).max() < 1e-8 * np.abs(rd).max()
+    np.testing.assert_allclose(ep.log_evidence(), dense.log_evidence(), rtol=1e-8)
+
+
+def test_state_evolution_sampling_and_tables(ctx):
+    "a table of D columns, positions of two axes; SE against the dense channel of the same matrix"
+    import tramp_amd as T
+    rs = np.random.RandomState(4)
+    V, D = 30, 3
+    tok = zipf_tokens(rs, V, 40, 0.5).reshape(8, 5)
+    W = dense_of(tok, V, D, 0.9)
+    lk = T.LookupChannel(tok, V, dim=D, scale=0.9, ctx=ctx)
+    model = (T.GaussianPrior(size=(V, D), ctx=ctx) @ T.SISOVariable(id="x") @ lk @ T.SISOVariable(id="z")
+             @ T.GaussianChannel(var=0.2) @ T.SILeafVariable(id="y")).to_model()
+    s = model.sample(seed=3)
+    assert s["z"].shape == (8, 5, D) and np.allclose(s["z"].reshape(-1), W @ s["x"].reshape(-1), rtol=1e-15, atol=0)
+    assert model.init_shapes()["z"] == (8, 5, D)
+    model.init_second_moments()
+    lin = orc.LinearOracle(W)
+    assert model.get_second_moments()["z"] == pytest.approx(lin.second_moment(1.0), rel=1e-12)
+    for az, ax in ((0.3, 2.0), (5.0, 0.0), (1.0, 40.0)):
+        assert lk.compute_forward_error(az, ax, 1.0) == pytest.approx(lin.forward_variance(az, ax), rel=1e-9)
+        assert lk.compute_backward_error(az, ax, 1.0) == pytest.approx(lin.backward_variance(az, ax), rel=1e-9)
+    obs = model.to_observed({"y": s["y"]})
+    ep = T.ExpectationPropagation(obs, ctx=ctx)
+    ep.iterate(max_iter=60, damping=0.1)
+    # Gaussian prior and noise: EP's fixed point is the exact posterior mean
+    H = W.T @ W / 0.2 + np.eye(V * D)
+    want = np.linalg.solve(H, W.T @ s["y"].reshape(-1) / 0.2)
+    assert np.abs(ep.get_variables_data()["x"]["r"].reshape(-1) - want).max() < 1e-4 * np.abs(want).max()
+    se = T.StateEvolution(obs)
+    se.iterate(max_iter=50)
+    assert 0 < se.get_variables_data()["x"]["v"] < 1
+
+
+def test_a_channel_made_on_one_context_runs_on_another(ctx):
+    import tramp_amd as T
+    rs = np.random.RandomState(6)
+    tok = zipf_tokens(rs, 20, 50, 0.5)
+    y = rs.standard_normal(50)
+    lk = T.LookupChannel(tok, 20, ctx=ctx)
+    want = T.ExpectationPropagation(regression(T, ctx, lk, 20, y), ctx=ctx).iterate(max_iter=5, callback=T.PassCallback()).get_variables_data()["x"]["r"]
+    other = T.Context(0)
+    lk2 = T.LookupChannel(tok, 20, ctx=ctx)
+    got = T.ExpectationPropagation(regression(T, other, lk2, 20, y), ctx=other).iterate(max_iter=5, callback=T.PassCallback()).get_variables_data()["x"]["r"]
+    assert np.array_equal(want, got)
+    del lk2

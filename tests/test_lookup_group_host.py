@@ -1,0 +1,164 @@
+"""Refusals of the lookup channel, of the array lists and of iterate(max_step=...) that need no device, and the plain
+definitions the GPU tests compare with, checked against the dense oracle of the linear channel."""
+import ctypes as C
+
+import numpy as np
+import pytest
+
+import tramp_amd as T
+from oracle import tramp_oracle as orc
+from tests.lookup_plain import LookupFactor, clip_plain, dense_of, step_plain
+
+
+class HostContext:
+    "stands where a context goes; the checks under test raise before any call"
+    device = 0
+    handle = None
+
+    def _call(self, name, *args):
+        raise AssertionError(f"{name} was reached")
+
+    def release(self, name, handle):
+        pass
+
+
+def fake(ctx, shape, dtype=np.float64, ptr=4096):
+    return T.DeviceArray(ctx, shape, dtype, ptr=ptr, owner=False)
+
+
+@pytest.mark.parametrize("kw, error", [
+    (dict(tokens=[0.5, 1.0], n_tokens=3), TypeError),
+    (dict(tokens=[True, False], n_tokens=3), TypeError),
+    (dict(tokens=np.zeros(0, int), n_tokens=3), ValueError),
+    (dict(tokens=[0, 3], n_tokens=3), ValueError),
+    (dict(tokens=[0, -1], n_tokens=3), ValueError),
+    (dict(tokens=[0, -2], n_tokens=3, padding_index=-1), ValueError),
+    (dict(tokens=[0, 2**40], n_tokens=3), ValueError),
+    (dict(tokens=[0], n_tokens=0), ValueError),
+    (dict(tokens=[0], n_tokens=3, dim=0), ValueError),
+    (dict(tokens=[0], n_tokens=2**31), ValueError),
+    (dict(tokens=[0], n_tokens=3, scale=0.0), ValueError),
+    (dict(tokens=[0], n_tokens=3, scale=np.nan), ValueError),
+    (dict(tokens=[0], n_tokens=3, scale=np.inf), ValueError),
+    (dict(tokens=[0], n_tokens=3, dtype=np.float16), ValueError),
+])
+def test_lookup_channel_refuses(kw, error):
+    with pytest.raises(error):
+        T.LookupChannel(ctx=HostContext(), **kw)
+
+
+def test_valid_arguments_reach_the_library():
+    with pytest.raises(AssertionError, match="tramp_lookup_create"):
+        T.LookupChannel([[0, 2], [7, 1]], 3, dim=2, padding_index=7, ctx=HostContext())
+    with pytest.raises(AssertionError, match="tramp_lookup_create"):
+        T.get_channel("lookup", tokens=np.uint8([0, 1]), n_tokens=2, ctx=HostContext())
+
+
+def test_array_group_refuses():
+    ctx, other = HostContext(), HostContext()
+    a = fake(ctx, (2, 5))
+    for arrays in ([], [np.zeros((2, 5))], [a, fake(ctx, (3, 5), ptr=1 << 20)], [a, fake(ctx, (2, 5), np.float32, ptr=1 << 20)],
+                   [a, fake(other, (2, 5), ptr=1 << 20)], [fake(ctx, (1, 2, 5))], [fake(ctx, (4,), np.uint8)]):
+        with pytest.raises(ValueError):
+            T.ArrayGroup(arrays)
+    with pytest.raises(AssertionError, match="tramp_group_create"):
+        T.ArrayGroup([a, fake(ctx, (2, 7), ptr=1 << 20)])
+
+
+def make_group(ctx, lengths, batch=2, dtype=np.float64):
+    g = T.ArrayGroup.__new__(T.ArrayGroup)
+    g.ctx, g.dtype, g.batch, g.lengths, g._handle = ctx, np.dtype(dtype), batch, tuple(lengths), C.c_void_p()
+    g.arrays = [fake(ctx, (batch, n)) for n in lengths]
+    return g
+
+
+def test_group_calls_refuse():
+    ctx = HostContext()
+    g = make_group(ctx, (4, 5))
+    norm = fake(ctx, (2,))
+    for bad in (0.0, -1.0, np.nan):
+        with pytest.raises(ValueError):
+            g.clip(bad, norm=norm)
+        with pytest.raises(ValueError):
+            g.limit_step(make_group(ctx, (4, 5)), bad, norm=norm)
+    for other in (make_group(ctx, (4, 6)), make_group(ctx, (4,)), make_group(ctx, (4, 5), batch=3), make_group(ctx, (4, 5), dtype=np.float32),
+                  make_group(HostContext(), (4, 5)), [1, 2]):
+        with pytest.raises(ValueError):
+            g.clip(1.0, out=other, norm=norm)
+        with pytest.raises(ValueError):
+            g.limit_step(other, 1.0, norm=norm)
+    for bad_norm in (fake(ctx, (3,)), fake(ctx, (2,), np.float32), np.zeros(2), fake(HostContext(), (2,))):
+        with pytest.raises(ValueError):
+            g.norm(bad_norm)
+    prev = make_group(ctx, (4, 5))
+    with pytest.raises(ValueError):
+        g.limit_step(prev, 1.0, norm=norm, a=fake(ctx, (3, 2)))
+    for a in (fake(ctx, (3, 4)), fake(ctx, (3, 2), np.float32), np.zeros((3, 2))):
+        with pytest.raises(ValueError):
+            g.limit_step(prev, 1.0, norm=norm, a=a, a_prev=fake(ctx, (3, 2)))
+
+
+def test_c_entries_refuse_a_null_context():
+    lib = T._lib.load()
+    h = C.c_void_p()
+    assert lib.tramp_lookup_create(None, 1, 2, 1, 1, None, 1.0, C.byref(h)) == T._lib.EINVAL
+    assert lib.tramp_lookup_apply(None, None, 1, None, None) == T._lib.EINVAL
+    assert lib.tramp_lookup_gradient(None, None, 1, None, None) == T._lib.EINVAL
+    assert lib.tramp_lookup_message(None, None, 0, 1, None, None, None, None, 0.0, None, None, None, None, None, None) == T._lib.EINVAL
+    assert lib.tramp_lookup_variance(None, None, 0, 1, None, None, None, None, None) == T._lib.EINVAL
+    assert lib.tramp_lookup_log_partition(None, None, 1, None, None, None, None, None) == T._lib.EINVAL
+    assert lib.tramp_lookup_destroy(None, None) == T._lib.EINVAL
+    assert lib.tramp_group_create(None, 1, 1, None, None, 1, C.byref(h)) == T._lib.EINVAL
+    assert lib.tramp_group_norm(None, None, None) == T._lib.EINVAL
+    assert lib.tramp_group_clip(None, None, 1.0, None, None) == T._lib.EINVAL
+    assert lib.tramp_group_limit_step(None, None, None, 1.0, None, 0, 0, None, None, None) == T._lib.EINVAL
+    assert lib.tramp_group_destroy(None, None) == T._lib.EINVAL
+
+
+def test_iterate_refuses_bad_steps():
+    ep = object.__new__(T.ExpectationPropagation)
+    ep.default_stopping = T.EarlyStoppingEP()
+    for bad in (0, -1.0, np.nan, True, "adaptive", [1.0]):
+        with pytest.raises(ValueError):
+            ep.iterate(max_step=bad)
+    with pytest.raises(ValueError):
+        ep.iterate(max_step=1.0, damping="adaptive")
+
+
+# ---------------------------------------------------------------- the plain definitions against the dense oracle
+@pytest.mark.parametrize("V, T_, pad", [(6, 17, 0), (9, 4, 1), (1, 3, 1), (5, 1, 0)])
+@pytest.mark.parametrize("scale", [1.0, -2.5])
+def test_plain_lookup_is_the_linear_channel_of_its_matrix(V, T_, pad, scale):
+    rs = np.random.RandomState(V * T_)
+    tok = rs.randint(0, V, T_)
+    if pad and T_ > 1:
+        tok[1] = -1
+    W = dense_of(tok, V, 1, scale)
+    lin, lk = orc.LinearOracle(W), LookupFactor(tok, V, 1, scale)
+    bz, bx = rs.standard_normal(V), rs.standard_normal(T_)
+    for az, ax in [(1.3, 0.7), (0.2, 5.0), (2.0, 0.0), (1e-3, 1e3)]:
+        for d in ("forward", "backward"):
+            a, b = getattr(lin, d + "_message")(az, bz, ax, bx)
+            a2, b2 = getattr(lk, d)(az, bz, ax, bx)
+            np.testing.assert_allclose(a2, a, rtol=1e-8, atol=1e-11)
+            np.testing.assert_allclose(b2, b, rtol=1e-8, atol=1e-8 * (np.abs(b).max() + 1))
+        assert lk.log_partition(az, bz, ax, bx) == pytest.approx(orc.linear_log_partition(lin, az, bz, ax, bx), rel=1e-10)
+        assert lk.n_eff(az, ax) == pytest.approx(lin.n_eff(az, ax), rel=1e-10, abs=1e-14)
+    assert lk.second_moment(0.7) == pytest.approx(lin.second_moment(0.7), rel=1e-12)
+
+
+def test_plain_clip_and_step():
+    rs = np.random.RandomState(0)
+    x = [rs.standard_normal((3, n)) for n in (4, 7)]
+    p = [rs.standard_normal((3, n)) for n in (4, 7)]
+    norm, y = clip_plain(x, 2.0)
+    np.testing.assert_allclose(norm, np.linalg.norm(np.concatenate(x, axis=1), axis=1))
+    np.testing.assert_allclose(np.linalg.norm(np.concatenate(y, axis=1), axis=1), np.minimum(norm, 2.0))
+    norm, y, c = step_plain(x, p, 1.5)
+    np.testing.assert_allclose(np.linalg.norm(np.concatenate(y, axis=1) - np.concatenate(p, axis=1), axis=1), np.minimum(norm, 1.5))
+    x[0][1, 2], x[1][2, 0] = np.nan, np.inf
+    norm, y = clip_plain(x, 1e-3)
+    assert np.isnan(norm[1]) and np.isinf(norm[2])
+    for b in (1, 2):
+        for u, w in zip(x, y):
+            np.testing.assert_array_equal(u[b], w[b])

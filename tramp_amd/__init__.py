@@ -10,6 +10,7 @@ There is no CPU fallback: without the built HIP library the compute methods rais
 """
 from . import _lib
 from .device import Context, DeviceArray, default_context
+from .group import ArrayGroup
 from .priors import (GaussBernoulliPrior, MAP_L1NormPrior, MAP_L21NormPrior, BinaryPrior, GaussianPrior, ExponentialPrior,
                      PositivePrior, GaussianMixturePrior, get_prior)
 from . import switches
@@ -19,7 +20,7 @@ from .likelihoods import (GaussianLikelihood, SgnLikelihood, AbsLikelihood, Asym
 from .channels import (LinearChannel, SolveLinearChannel, ComplexLinearChannel, ModulusChannel, SgnChannel, AbsChannel, ReluChannel, GaussianChannel,
                        LeakyReluChannel, AsymmetricAbsChannel, HardTanhChannel, HardSigmoidChannel,
                        SymmetricDoorChannel, ConvChannel, Blur1DChannel, Blur2DChannel,
-                       DifferentialChannel, LaplacianChannel, DFTChannel, RotationChannel, GradientChannel, UnitaryChannel, ReshapeChannel, BiasChannel, SumChannel, DuplicateChannel,
+                       DifferentialChannel, LaplacianChannel, DFTChannel, RotationChannel, GradientChannel, LookupChannel, UnitaryChannel, ReshapeChannel, BiasChannel, SumChannel, DuplicateChannel,
                        MarchenkoPasturChannel, AnalyticalLinearChannel, get_channel)
 from .variables import SISOVariable, SILeafVariable, SIMOVariable, MISOVariable, MILeafVariable
 from .models import (Model, DAG, MultiLayerModel, glm_generative, glm_state_evolution,

@@ -105,6 +105,18 @@ _SIGNATURES = {
     "tramp_grad_variance": [vp, vp, i32, sz, vp, vp, vp, vp, vp],
     "tramp_grad_apply": [vp, vp, sz, vp, vp],
     "tramp_grad_message": [vp, vp, i32, sz, vp, vp, vp, vp, dbl, vp, vp, vp, vp, vp, vp, i32],
+    "tramp_lookup_create": [vp, i32, sz, sz, sz, vp, dbl, C.POINTER(vp)],
+    "tramp_lookup_destroy": [vp, vp],
+    "tramp_lookup_apply": [vp, vp, sz, vp, vp],
+    "tramp_lookup_gradient": [vp, vp, sz, vp, vp],
+    "tramp_lookup_variance": [vp, vp, i32, sz, vp, vp, vp, vp, vp],
+    "tramp_lookup_message": [vp, vp, i32, sz, vp, vp, vp, vp, dbl, vp, vp, vp, vp, vp, vp],
+    "tramp_lookup_log_partition": [vp, vp, sz, vp, vp, vp, vp, vp],
+    "tramp_group_create": [vp, i32, i32, C.POINTER(vp), C.POINTER(sz), sz, C.POINTER(vp)],
+    "tramp_group_destroy": [vp, vp],
+    "tramp_group_norm": [vp, vp, vp],
+    "tramp_group_clip": [vp, vp, dbl, vp, vp],
+    "tramp_group_limit_step": [vp, vp, vp, dbl, vp, i32, sz, vp, vp, vp],
     "tramp_linear_set_rotated": [vp, vp, i32],
     "tramp_lsolve_create": [vp, i32, sz, sz, vp, C.POINTER(vp)],
     "tramp_lsolve_destroy": [vp, vp],

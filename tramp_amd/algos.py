@@ -619,14 +619,14 @@ class ExpectationPropagation:
 
     def _moment_hint(self, i):
         "the prior that consumes the backward message into variable i, if it can use fused moments"
-        if i in self._rot:
+        if i in self._rot or self._max_step:
             return None                 # the stored message lives in a rotated basis
         f = self.model.prev_factor(self.variables[i])
         return f.moment_hint() if f.n_prev == 0 and hasattr(f, "moment_hint") else None
 
     def _lik_hint(self, i, n):
         "the likelihood that consumes the forward message into variable i, if it can use fused moments"
-        if i in self._rot:
+        if i in self._rot or self._max_step:
             return None
         f = self.model.next_factor(self.variables[i])
         return f.lik_hint(self.batch, n) if f is not None and f.n_next == 0 and hasattr(f, "lik_hint") else None
@@ -878,6 +878,44 @@ class ExpectationPropagation:
         self.ctx._call("tramp_prior_hint", 0, 0.0, 0.0, 0.0, 0, 0, None, None)
         self._const_done = set()
 
+    # -- bounded steps (iterate(max_step=...)): after the two sweeps of an iteration every message m becomes
+    # m_old + c (m - m_old), c = min(1, max_step / |b - b_old|) with the norm over the b of ALL messages of one instance
+    # (csrc/group.hip) - constant damping (message_passing.py:119-127) with a factor per instance and iteration.  The old
+    # messages are the previous set of the alternating buffers where there is one, else a copy that the same launch refreshes.
+    _max_step = None
+
+    def _step_buffers(self):
+        "(b vectors, precision table) of the live messages, every buffer once"
+        return self.b_fwd + self.b_bwd, self.A
+
+    def _step_buffers_prev(self):
+        return self._snap["fwd"] + self._snap["bwd"], self._snap["A"]
+
+    def _step_setup(self):
+        from .group import ArrayGroup
+        ctx = self.ctx
+        # moments left for a consumer belong to messages that will be rewritten
+        ctx._call("tramp_prior_hint", 0, 0.0, 0.0, 0.0, 0, 0, None, None)
+        self._const_done = set()
+        live, A = self._step_buffers()
+        if self._pp_active():
+            prev, A_prev = self._step_buffers_prev()
+        else:
+            prev = [ctx.empty(tuple(b.shape), self.dtype).copy_from(b) for b in live]
+            A_prev = ctx.empty(tuple(A.shape), np.float64).copy_from(A)
+        self._step_lists = {live[0].ptr: ArrayGroup(live, ctx=ctx), prev[0].ptr: ArrayGroup(prev, ctx=ctx)}
+        self._step_saved = None if self._pp_active() else (prev, A_prev)
+        self.step_norm = ctx.zeros((self.batch,), np.float64)
+
+    def _bound_step(self):
+        live, A = self._step_buffers()
+        prev, A_prev = self._step_saved or self._step_buffers_prev()
+        self._step_lists[live[0].ptr].limit_step(self._step_lists[prev[0].ptr], self._max_step, norm=self.step_norm, a=A,
+                                                 a_prev=A_prev, refresh=self._step_saved is not None)
+        for b in live:
+            b.version += 1
+        self._const_done = set()             # a constant message is on its way to its value, not there
+
     def _poll_monitor(self):
         """Read the state words; raises on a NaN message (message_passing.py:187-209), otherwise updates
         status / n_iter_instance / frozen scalars and returns the number of instances still running."""
@@ -1095,6 +1133,8 @@ class ExpectationPropagation:
             self._take_snapshot()
         self.forward_message()
         self.backward_message()
+        if self._max_step:
+            self._bound_step()
         self.update_variables()
         if mon is not None:
             self._monitor_step(*mon)
@@ -1125,7 +1165,7 @@ class ExpectationPropagation:
         return stop[0], [cb for cb in members if cb is not stop[0] and type(cb) is not PassCallback]
 
     def iterate(self, max_iter=200, callback=None, initializer=None, damping=None, warm_start=False,
-                check_every=1, graph=False, restore_messages=None, update_dA=False):
+                check_every=1, graph=False, restore_messages=None, update_dA=False, max_step=None):
         """message_passing.py:330-357.  The NaN guard and the per-instance stopping rule run on the device
         after every iteration (csrc/monitor.hip); ``check_every`` = k makes the host look at their state
         words - and run the remaining host callbacks - only every k-th iteration, the sweeps themselves
@@ -1140,12 +1180,21 @@ class ExpectationPropagation:
         an instance that gives up after an increase gets the previous iteration's messages back, a converged one
         keeps those of its stopping iteration, and a NaN puts every instance back one iteration before ValueError
         is raised (message_passing.py:187-209, callbacks.py:233-240,277-283); a warm start then continues each
-        instance from where its own run would have stopped."""
+        instance from where its own run would have stopped.
+        ``max_step`` bounds the step of an iteration: the norm of new minus old b over all messages of an instance; a
+        longer step is shortened to it, precisions included, on top of constant damping.  ``step_norm`` holds the norms
+        before the bound, per instance (double[batch] on the device, of the last iteration)."""
         if update_dA:
             raise NotImplementedError("update_dA (the per-message free-energy increments of message_passing.py:245-246) is not tracked")
         initializer = initializer or ConstantInit(a=0, b=0)
         callback = callback or self.default_stopping
         adaptive = isinstance(damping, str) and damping == "adaptive"
+        if max_step is not None:
+            if isinstance(max_step, bool) or not isinstance(max_step, (int, float, np.integer, np.floating)) or not max_step > 0:
+                raise ValueError(f"max_step must be None or a positive number, got {max_step!r}")
+            if adaptive:
+                raise ValueError("max_step and adaptive damping exclude each other")
+            max_step = float(max_step)
         if isinstance(damping, (int, np.integer, np.floating)) and not isinstance(damping, bool):
             damping = float(damping)                           # the reference's examples pass damping=0
         if damping is not None and damping is not False and not isinstance(damping, float) and not adaptive:
@@ -1199,6 +1248,7 @@ class ExpectationPropagation:
                              (restore_messages if restore_messages is not None else stopper is not None))
         if self._restore and getattr(self, "_snap", None) is None:
             self._allocate_snapshot()
+        self._max_step = max_step
         n0 = self._n0 = self.n_iter
         period = 2 if mon is not None else 1           # r / r_prev ping-pong: the launch sequence has period two
         graphs = {}
@@ -1207,6 +1257,8 @@ class ExpectationPropagation:
         if self._pp_active():
             self._sync_snapshot()
         try:
+            if max_step:
+                self._step_setup()
             i = 0
             while i < max_iter:
                 par = i % period
@@ -1248,6 +1300,7 @@ class ExpectationPropagation:
             basis.__exit__(None, None, None)
             for g in graphs.values():
                 self.ctx._call("tramp_graph_destroy", g)
+            self._step_lists = self._step_saved = None
         if self._restore and stopper is not None and self.status.any():
             self._restore_messages()
         if stopper is not None and self.status.all():

@@ -1482,6 +1482,170 @@ class GradientChannel(Channel):
     compute_backward_message = ConvChannel.compute_backward_message
 
 
+class LookupChannel(Channel):
+    """Lookup channel x_t = scale z[token_t]: the linear channel of categorical data.
+
+    ``tokens`` is an integer array of any shape, the row of the table z each position reads; z is a vector of ``n_tokens``
+    (``dim=None``) or a table [n_tokens, dim], x has the shape of ``tokens`` (+ ``(dim,)``).  Positions that hold
+    ``padding_index`` read nothing (x = 0 there, a zero row of the matrix).  The same channel as ``LinearChannel`` of the
+    one-hot design matrix times ``scale`` (tramp/channels/linear/linear_channel.py:18-132), without the matrix: the positions
+    are sorted by token once, W^T W is diagonal with entries scale^2 count, variances and messages are closed forms in the
+    counts (csrc/lookup.hip).  Device vectors: z [batch, n_tokens dim], x [batch, positions dim].
+    """
+
+    def __init__(self, tokens, n_tokens, dim=None, scale=1.0, padding_index=None, name="E", dtype=np.float64, ctx=None):
+        tok = np.asarray(tokens)
+        if tok.dtype.kind not in "iu":
+            raise TypeError(f"tokens must be integers, got {tok.dtype}")
+        self.n_tokens, self.dim = int(n_tokens), None if dim is None else int(dim)
+        if self.n_tokens < 1 or (self.dim is not None and self.dim < 1):
+            raise ValueError(f"the table needs a row and a column, got n_tokens={n_tokens}, dim={dim}")
+        if tok.size < 1:
+            raise ValueError("tokens is empty")
+        cols = self.dim or 1
+        if max(tok.size, self.n_tokens, cols) >= 2**31 - 1:
+            raise ValueError("positions, rows and columns must stay below 2^31 - 1")
+        scale = float(scale)
+        if not np.isfinite(scale) or scale == 0.0:
+            raise ValueError(f"scale must be finite and not zero, got {scale}")
+        padded = np.zeros(tok.shape, dtype=bool) if padding_index is None else tok == padding_index
+        read = tok[~padded]
+        if read.size and (read.min() < 0 or read.max() >= self.n_tokens):
+            raise ValueError(f"tokens must lie in [0, {self.n_tokens}), got [{read.min()}, {read.max()}]")
+        self.scale, self.padding_index, self.name = scale, padding_index, name
+        self.repr_init()
+        self._init_device(dtype, ctx)
+        self._zshape = (self.n_tokens,) if self.dim is None else (self.n_tokens, self.dim)
+        self._xshape = tok.shape + (() if self.dim is None else (self.dim,)) or (1,)
+        self.Nz, self.Nx = self.n_tokens * cols, tok.size * cols
+        self.alpha = self.Nx / self.Nz
+        host = np.ascontiguousarray(np.where(padded, -1, tok).reshape(-1), dtype=np.int32)
+        self._seen = int(read.size)
+        self._tokens_h = host
+        h = C.c_void_p()
+        self.ctx._call("tramp_lookup_create", self._dt, self.n_tokens, cols, tok.size, host.ctypes.data, scale, C.byref(h))
+        self._handle = h
+
+    def __del__(self):
+        try:
+            self.ctx.release("tramp_lookup_destroy", self._handle)
+        except Exception:
+            pass
+        self._handle = None
+
+    def _vec(self, b, x_side):
+        n = self.Nx if x_side else self.Nz
+        if isinstance(b, DeviceArray):
+            if b.ctx is not self.ctx:
+                raise ValueError("device array of another context")
+            arg = VecArg(self.ctx, b, self.dtype)
+            if arg.n != n:
+                raise ValueError(f"expected {'bx' if x_side else 'bz'} of [batch,{n}], got {b.shape}")
+            return arg
+        full = self._xshape if x_side else self._zshape
+        h = np.asarray(b, dtype=self.dtype)
+        nd = len(full)
+        if h.shape[-nd:] != full or h.ndim not in (nd, nd + 1):
+            raise ValueError(f"expected an array of shape {full} or (batch,)+{full}, got {h.shape}")
+        arg = VecArg(self.ctx, h.reshape(-1, n) if h.ndim == nd + 1 else h.reshape(n), self.dtype)
+        arg.host_shape = h.shape
+        arg._one = h.ndim == nd
+        return arg
+
+    def _out(self, out, batch, n, dtype):
+        "the caller's result buffer, checked, or a new one"
+        if out is None:
+            return self.ctx.empty((batch, n), dtype)
+        if not isinstance(out, DeviceArray) or out.ctx is not self.ctx or out.dtype != np.dtype(dtype) or out.size != batch * n:
+            raise ValueError(f"the result needs a device array of {batch} x {n} {np.dtype(dtype)} in this context, got {out!r}")
+        return out
+
+    _ret = staticmethod(ConvChannel._ret)
+    _ret_scal = staticmethod(ConvChannel._ret_scal)
+
+    def _linear(self, entry, src, x_side, out):
+        v = self._vec(src, x_side)
+        full, n = (self._zshape, self.Nz) if x_side else (self._xshape, self.Nx)
+        dev = self._out(out, v.batch, n, self.dtype)
+        self.ctx._call(entry, self._handle, v.batch, v.dev.ptr, dev.ptr)
+        if out is not None or not v.was_host:
+            return dev
+        return dev.get().reshape(full if v._one else (v.batch,) + full)
+
+    def lookup(self, z, out=None):
+        "x = scale z[tokens], 0 at padded positions"
+        return self._linear("tramp_lookup_apply", z, False, out)
+
+    def gradient(self, x, out=None):
+        "the adjoint: row v is scale times the sum of x over the positions of token v, added in the order of the positions"
+        return self._linear("tramp_lookup_gradient", x, True, out)
+
+    def sample(self, Z):
+        return self.lookup(Z)
+
+    def second_moment(self, tau_z):
+        return tau_z * self.scale**2 * self._seen / self._tokens_h.size             # linear_channel.py:55-56
+
+    def device_variance(self, direction, az, ax):
+        "(v, a_new, n_eff) on the device for a batch of (az, ax)"
+        ctx = self.ctx
+        az_h = np.atleast_1d(np.asarray(az, dtype=np.float64))
+        a_z = ctx.scalars(az_h)
+        a_x = ctx.scalars(ax, az_h.shape[0])
+        outs = [ctx.empty((az_h.shape[0],), np.float64) for _ in range(3)]
+        ctx._call("tramp_lookup_variance", self._handle, direction, az_h.shape[0], a_z.ptr, a_x.ptr, *[o.ptr for o in outs])
+        return [o.get() for o in outs]
+
+    def compute_n_eff(self, az, ax):
+        return float(self.device_variance(_lib.FWD, az, ax)[2][0])
+
+    def compute_backward_variance(self, az, ax):
+        return float(self.device_variance(_lib.BWD, az, ax)[0][0])
+
+    def compute_forward_variance(self, az, ax):
+        return float(self.device_variance(_lib.FWD, az, ax)[0][0])
+
+    def compute_backward_error(self, az, ax, tau_z):
+        return self.compute_backward_variance(az, ax)
+
+    def compute_forward_error(self, az, ax, tau_z):
+        return self.compute_forward_variance(az, ax)
+
+    def _args(self, az, bz, ax, bx):
+        z, x = self._vec(bz, False), self._vec(bx, True)
+        if z.batch != x.batch:
+            raise ValueError(f"bz holds {z.batch} instances, bx {x.batch}")
+        return z, x, ScalArg(self.ctx, az, z.batch), ScalArg(self.ctx, ax, z.batch)
+
+    def _run(self, direction, az, bz, ax, bx, out_a=None, out_b=None, damping=0.0, old_a=None, old_b=None, want_posterior=False):
+        ctx = self.ctx
+        z, x, a_z, a_x = self._args(az, bz, ax, bx)
+        tgt, a_t = (x, a_x) if direction == _lib.FWD else (z, a_z)
+        a_new = out_a if out_a is not None else ctx.empty((z.batch,), np.float64)
+        b_new = self._out(out_b, z.batch, tgt.n, self.dtype)
+        r = ctx.empty((z.batch, tgt.n), self.dtype) if want_posterior else None
+        v = ctx.empty((z.batch,), np.float64) if want_posterior else None
+        ctx._call("tramp_lookup_message", self._handle, direction, z.batch, a_z.dev.ptr, z.dev.ptr, a_x.dev.ptr, x.dev.ptr,
+                  float(damping or 0.0), old_a.ptr if old_a is not None else None, old_b.ptr if old_b is not None else None,
+                  a_new.ptr, b_new.ptr, r.ptr if r is not None else None, v.ptr if v is not None else None)
+        return tgt, a_t, a_new, b_new, r, v
+
+    compute_backward_mean = ConvChannel.compute_backward_mean
+    compute_forward_mean = ConvChannel.compute_forward_mean
+    compute_backward_posterior = ConvChannel.compute_backward_posterior
+    compute_forward_posterior = ConvChannel.compute_forward_posterior
+    compute_forward_message = ConvChannel.compute_forward_message
+    compute_backward_message = ConvChannel.compute_backward_message
+
+    def compute_log_partition(self, az, bz, ax, bx):
+        "linear_channel.py:127-132"
+        z, x, a_z, a_x = self._args(az, bz, ax, bx)
+        out = self.ctx.empty((z.batch,), np.float64)
+        self.ctx._call("tramp_lookup_log_partition", self._handle, z.batch, a_z.dev.ptr, z.dev.ptr, a_x.dev.ptr, x.dev.ptr, out.ptr)
+        res = out.get()
+        return float(res[0]) if (a_z.was_host and a_z.scalar_like and z.was_host and z._one) else res
+
+
 class _UnitaryChannel(Channel):
     """Shared message plumbing of the unitary channels (DFT, rotation): the posterior is not
     needed - (a, b) travel through the change of basis (a unchanged, b transformed)."""
@@ -1853,6 +2017,7 @@ CHANNEL_CLASSES = {
     "dft": DFTChannel,
     "rotation": RotationChannel,
     "gradient": GradientChannel,
+    "lookup": LookupChannel,
     "unitary": UnitaryChannel,
     "reshape": ReshapeChannel,
     "bias": BiasChannel,

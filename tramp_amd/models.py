@@ -11,7 +11,7 @@ import networkx as nx
 import numpy as np
 
 from .base import Factor, Variable
-from .channels import (AsymmetricAbsChannel, ConvChannel, DFTChannel, GradientChannel, ReshapeChannel, GaussianChannel, HardTanhChannel, HardSigmoidChannel, SymmetricDoorChannel, SgnChannel, AbsChannel, ReluChannel, LeakyReluChannel, LinearChannel,
+from .channels import (AsymmetricAbsChannel, ConvChannel, DFTChannel, GradientChannel, LookupChannel, ReshapeChannel, GaussianChannel, HardTanhChannel, HardSigmoidChannel, SymmetricDoorChannel, SgnChannel, AbsChannel, ReluChannel, LeakyReluChannel, LinearChannel,
                        ComplexLinearChannel, ModulusChannel, PiecewiseLinearChannel, get_channel)
 from .ensembles import get_ensemble
 from .likelihoods import (GaussianLikelihood, SgnLikelihood, AbsLikelihood, AsymmetricAbsLikelihood, ReluLikelihood,
@@ -229,6 +229,8 @@ class Model:
         if isinstance(factor, ConvChannel):
             # real=False: planar complex vectors (2,) + shape (channels.py ConvChannel._vshape)
             return tuple(factor._vshape)
+        if isinstance(factor, LookupChannel):
+            return tuple(factor._xshape)
         if isinstance(factor, GradientChannel):
             return (factor.d,) + tuple(factor.shape)
         if isinstance(factor, DFTChannel):

@@ -219,6 +219,13 @@ class TreeExpectationPropagation(ExpectationPropagation):
         self.A, self._snap["A"] = self._snap["A"], self.A
         self._written = set()
 
+    def _step_buffers(self):
+        "every message of both directions once (an aliased message is the other side's buffer)"
+        return [self.msg[k].b for k in self.msg_keys if k not in self._aliased], self.A
+
+    def _step_buffers_prev(self):
+        return [self._msg_prev[k].b for k in self.msg_keys if k not in self._aliased], self._snap["A"]
+
     # -- node updates
     def _factor_send(self, f, direction):
         g = self.model.dag
