@@ -2,10 +2,11 @@
 // bounded step new <- old + min(1, max / |new - old|) (new - old) of a whole set of EP messages.
 //
 // The arrays of a list have lengths of their own, [batch, n_i] each; an instance b owns row b of every array.  The list is laid
-// out once as chunks of kChunk elements that never straddle two arrays; workgroup p of instance b walks the chunks p, p + P, ...
-// and leaves one partial sum of squares, the second launch adds the P partials of its instance in a fixed order (every
-// workgroup for itself: P <= 1024 doubles out of the L2) and applies the factor.  Sums are held in double: no overflow below
-// 1e154, no loss in long sums, and the same bits every time.
+// out once as chunks of 32 KiB that never straddle two arrays; workgroup p of instance b walks the chunks p, p + P, ... and
+// leaves one partial sum of squares, the second launch adds the P partials of its instance in a fixed order (every workgroup
+// for itself: P <= 2048 doubles out of the L2) and applies the factor, from the last chunk to the first: what the first pass
+// read last is still in the 256 MB of cache before memory.  Sums are held in double: no overflow below 1e154, no loss in long
+// sums, and the same bits every time.
 #include "common.h"
 
 #include <algorithm>
@@ -13,9 +14,17 @@
 #include <vector>
 
 namespace {
-constexpr size_t kChunk = 4096;
-constexpr int kMaxPartials = 1024;
+constexpr size_t kChunkBytes = 32768;                // 8 pieces of 16 bytes per thread
+constexpr int kPieces = kChunkBytes / 16 / kBlock;
+constexpr int kMaxPartials = 2048;
 }  // namespace
+
+// one chunk: everything a workgroup needs in one scalar load, the next one's is on its way while this one is worked on
+struct GroupChunk {
+    unsigned long long addr;     // of its first element, instance 0
+    unsigned long long stride;   // bytes from one instance to the next
+    unsigned long long len;      // elements
+};
 
 struct tramp_group {
     int device;
@@ -24,38 +33,55 @@ struct tramp_group {
     size_t batch;
     size_t nchunk;
     void* mem;
-    void* const* ptr;            // [k] device pointers
-    const size_t* len;           // [k]
-    const int* chunk_array;      // [nchunk] the array a chunk belongs to
-    const unsigned* first;       // [k] the first chunk of every array
+    const GroupChunk* chunks;    // [nchunk]; lists of the same lengths have the same chunks
     void** ptr_h;                // host copies (checks between lists)
     size_t* len_h;
 };
 
-struct GroupDev {
-    void* const* ptr;
-    const size_t* len;
-    const int* chunk_array;
-    const unsigned* first;
-    unsigned nchunk;
+// 16-byte pieces at any element boundary
+template <typename T> struct GVec;
+template <> struct GVec<float> {
+    typedef float U __attribute__((ext_vector_type(4), aligned(4)));
+    static constexpr int N = 4;
 };
-
-static GroupDev dev_of(const tramp_group* g) { return GroupDev{g->ptr, g->len, g->chunk_array, g->first, (unsigned)g->nchunk}; }
+template <> struct GVec<double> {
+    typedef double U __attribute__((ext_vector_type(2), aligned(8)));
+    static constexpr int N = 2;
+};
 
 // partial sums of squares of x (STEP = false) or of x - prev
 template <typename T, bool STEP>
-__global__ __launch_bounds__(kBlock) void group_squares_kernel(GroupDev g, void* const* __restrict__ prev, double* __restrict__ partials) {
+__global__ __launch_bounds__(kBlock) void group_squares_kernel(unsigned nchunk, const GroupChunk* __restrict__ xs, const GroupChunk* __restrict__ ps,
+                                                               double* __restrict__ partials) {
+    using U = typename GVec<T>::U;
+    constexpr int N = GVec<T>::N;
+    constexpr size_t CH = kChunkBytes / sizeof(T);
     __shared__ double smem[kBlock / kWave];
     const size_t b = blockIdx.y;
     double acc = 0.0;
-    for (unsigned c = blockIdx.x; c < g.nchunk; c += gridDim.x) {
-        const int i = g.chunk_array[c];
-        const size_t n = g.len[i], lo = (size_t)(c - g.first[i]) * kChunk, hi = lo + kChunk < n ? lo + kChunk : n;
-        const T* x = static_cast<const T*>(g.ptr[i]) + b * n;
-        const T* p = STEP ? static_cast<const T*>(prev[i]) + b * n : nullptr;
-        for (size_t j = lo + threadIdx.x; j < hi; j += kBlock) {
-            const double d = STEP ? (double)x[j] - (double)p[j] : (double)x[j];
-            acc += d * d;
+    for (unsigned c = blockIdx.x; c < nchunk; c += gridDim.x) {
+        const T* x = reinterpret_cast<const T*>(xs[c].addr + b * xs[c].stride);
+        const T* p = STEP ? reinterpret_cast<const T*>(ps[c].addr + b * ps[c].stride) : nullptr;
+        const size_t len = xs[c].len;
+        if (len == CH) {
+            U v[kPieces], w[kPieces];
+#pragma unroll
+            for (int i = 0; i < kPieces; ++i) {
+                v[i] = reinterpret_cast<const U*>(x)[i * kBlock + threadIdx.x];
+                if (STEP) w[i] = reinterpret_cast<const U*>(p)[i * kBlock + threadIdx.x];
+            }
+#pragma unroll
+            for (int i = 0; i < kPieces; ++i)
+#pragma unroll
+                for (int e = 0; e < N; ++e) {
+                    const double d = STEP ? (double)v[i][e] - (double)w[i][e] : (double)v[i][e];
+                    acc = fma(d, d, acc);
+                }
+        } else {
+            for (size_t j = threadIdx.x; j < len; j += kBlock) {
+                const double d = STEP ? (double)x[j] - (double)p[j] : (double)x[j];
+                acc = fma(d, d, acc);
+            }
         }
     }
     acc = block_sum(acc, smem);
@@ -79,11 +105,20 @@ __global__ __launch_bounds__(kBlock) void group_norm_kernel(const double* __rest
     if (threadIdx.x == 0) norm_out[blockIdx.x] = n;
 }
 
-// out = c x, or out = prev + c (x - prev) with the precisions a moved by the same factor; REFRESH writes the result over prev too
+template <typename T, bool STEP> __device__ __forceinline__ T bounded(T x, T p, double c) {
+    if (c == 1.0) return x;
+    return STEP ? T((double)p + c * ((double)x - (double)p)) : T(c * (double)x);
+}
+
+// out = c x, or out = prev + c (x - prev) with the precisions a moved by the same factor; refresh: the result over prev too
 template <typename T, bool STEP>
-__global__ __launch_bounds__(kBlock) void group_apply_kernel(GroupDev g, void* const* prev, void* const* out, int refresh, double bound,
+__global__ __launch_bounds__(kBlock) void group_apply_kernel(unsigned nchunk, const GroupChunk* __restrict__ xs, const GroupChunk* __restrict__ ps,
+                                                             const GroupChunk* __restrict__ os, int refresh, double bound,
                                                              const double* __restrict__ partials, int P, size_t n_a, size_t B, double* a,
                                                              double* a_prev, double* __restrict__ norm_out) {
+    using U = typename GVec<T>::U;
+    constexpr int N = GVec<T>::N;
+    constexpr size_t CH = kChunkBytes / sizeof(T);
     __shared__ double smem[kBlock / kWave];
     const size_t b = blockIdx.y;
     const double norm = fold_norm(partials, P, b, smem), c = clip_factor(norm, bound);
@@ -97,18 +132,33 @@ __global__ __launch_bounds__(kBlock) void group_apply_kernel(GroupDev g, void* c
                 if (refresh) a_prev[i * B + b] = r;
             }
     }
-    for (unsigned ch = blockIdx.x; ch < g.nchunk; ch += gridDim.x) {
-        const int i = g.chunk_array[ch];
-        const size_t n = g.len[i], lo = (size_t)(ch - g.first[i]) * kChunk, hi = lo + kChunk < n ? lo + kChunk : n;
-        const T* x = static_cast<const T*>(g.ptr[i]) + b * n;
-        T* p = STEP ? static_cast<T*>(prev[i]) + b * n : nullptr;
-        T* o = static_cast<T*>(out[i]) + b * n;
+    for (unsigned k = blockIdx.x; k < nchunk; k += gridDim.x) {
+        const unsigned ch = nchunk - 1 - k;
+        const T* x = reinterpret_cast<const T*>(xs[ch].addr + b * xs[ch].stride);
+        T* p = STEP ? reinterpret_cast<T*>(ps[ch].addr + b * ps[ch].stride) : nullptr;
+        T* o = reinterpret_cast<T*>(os[ch].addr + b * os[ch].stride);
+        const size_t len = xs[ch].len;
         if (c == 1.0 && o == x && !(STEP && refresh)) continue;
-        for (size_t j = lo + threadIdx.x; j < hi; j += kBlock) {
-            T r = x[j];
-            if (c < 1.0) r = STEP ? T((double)p[j] + c * ((double)r - (double)p[j])) : T(c * (double)r);
-            o[j] = r;
-            if (STEP && refresh) p[j] = r;
+        if (len == CH) {
+            U v[kPieces], w[kPieces];
+#pragma unroll
+            for (int i = 0; i < kPieces; ++i) {
+                v[i] = reinterpret_cast<const U*>(x)[i * kBlock + threadIdx.x];
+                if (STEP) w[i] = reinterpret_cast<const U*>(p)[i * kBlock + threadIdx.x];
+            }
+#pragma unroll
+            for (int i = 0; i < kPieces; ++i) {
+#pragma unroll
+                for (int e = 0; e < N; ++e) v[i][e] = bounded<T, STEP>(v[i][e], STEP ? w[i][e] : T(0), c);
+                reinterpret_cast<U*>(o)[i * kBlock + threadIdx.x] = v[i];
+                if (STEP && refresh) reinterpret_cast<U*>(p)[i * kBlock + threadIdx.x] = v[i];
+            }
+        } else {
+            for (size_t j = threadIdx.x; j < len; j += kBlock) {
+                const T r = bounded<T, STEP>(x[j], STEP ? p[j] : T(0), c);
+                o[j] = r;
+                if (STEP && refresh) p[j] = r;
+            }
         }
     }
 }
@@ -122,14 +172,14 @@ extern "C" int tramp_group_create(tramp_ctx* ctx, int dtype, int k, void* const*
     TRAMP_REQUIRE(ctx, dtype == TRAMP_F32 || dtype == TRAMP_F64);
     TRAMP_REQUIRE(ctx, k >= 1 && arrays_d && n && batch >= 1 && batch <= 65535);
     TRAMP_REQUIRE(ctx, !ctx->capturing);
-    const size_t e = dtype_size(dtype);
+    const size_t e = dtype_size(dtype), per = kChunkBytes / e;
     try {
         size_t nchunk = 0;
         std::vector<std::pair<uintptr_t, uintptr_t>> span;
         for (int i = 0; i < k; ++i) {
             TRAMP_REQUIRE(ctx, arrays_d[i] || !n[i]);
             TRAMP_REQUIRE(ctx, n[i] <= ((size_t)1 << 40) / batch);
-            nchunk += (n[i] + kChunk - 1) / kChunk;
+            nchunk += (n[i] + per - 1) / per;
             const uintptr_t a = (uintptr_t)arrays_d[i];
             if (n[i]) span.emplace_back(a, a + n[i] * batch * e);
         }
@@ -138,21 +188,14 @@ extern "C" int tramp_group_create(tramp_ctx* ctx, int dtype, int k, void* const*
         for (size_t i = 1; i < span.size(); ++i)
             if (span[i].first < span[i - 1].second)
                 return tramp_fail(ctx, TRAMP_EINVAL, "tramp_group_create", "two arrays of the list overlap");
-        std::vector<int> chunk_array;
-        std::vector<unsigned> first((size_t)k);
-        chunk_array.reserve(nchunk);
-        for (int i = 0; i < k; ++i) {
-            first[(size_t)i] = (unsigned)chunk_array.size();
-            chunk_array.insert(chunk_array.end(), (n[i] + kChunk - 1) / kChunk, i);
-        }
-        auto up = [](size_t bytes) { return (bytes + 255) & ~(size_t)255; };
-        const size_t o_len = up((size_t)k * 8), o_first = o_len + up((size_t)k * 8), o_chunk = o_first + up((size_t)k * 4);
-        const size_t total = o_chunk + up(nchunk * 4);
-        std::vector<char> host(total, 0);
-        memcpy(host.data(), arrays_d, (size_t)k * 8);
-        memcpy(host.data() + o_len, n, (size_t)k * 8);
-        memcpy(host.data() + o_first, first.data(), (size_t)k * 4);
-        if (nchunk) memcpy(host.data() + o_chunk, chunk_array.data(), nchunk * 4);
+        std::vector<GroupChunk> chunks;
+        chunks.reserve(nchunk);
+        for (int i = 0; i < k; ++i)
+            for (size_t lo = 0; lo < n[i]; lo += per)
+                chunks.push_back(GroupChunk{(unsigned long long)(uintptr_t)arrays_d[i] + lo * e, (unsigned long long)(n[i] * e),
+                                            (unsigned long long)std::min(per, n[i] - lo)});
+        const size_t total = std::max(nchunk, (size_t)1) * sizeof(GroupChunk);
+        chunks.resize(std::max(nchunk, (size_t)1));
         tramp_group* g = new tramp_group();
         *g = tramp_group{};
         g->ptr_h = static_cast<void**>(malloc((size_t)k * 8));
@@ -165,7 +208,7 @@ extern "C" int tramp_group_create(tramp_ctx* ctx, int dtype, int k, void* const*
             delete g;
             return tramp_fail(ctx, TRAMP_ENOMEM, "tramp_group_create", "out of memory");
         }
-        hipError_t err = hipMemcpyAsync(g->mem, host.data(), total, hipMemcpyHostToDevice, ctx->stream);
+        hipError_t err = hipMemcpyAsync(g->mem, chunks.data(), total, hipMemcpyHostToDevice, ctx->stream);
         if (err == hipSuccess) err = hipStreamSynchronize(ctx->stream);
         if (err != hipSuccess) {
             (void)hipFree(g->mem);
@@ -176,16 +219,12 @@ extern "C" int tramp_group_create(tramp_ctx* ctx, int dtype, int k, void* const*
         }
         memcpy(g->ptr_h, arrays_d, (size_t)k * 8);
         memcpy(g->len_h, n, (size_t)k * 8);
-        char* m = static_cast<char*>(g->mem);
         g->device = ctx->device;
         g->dtype = dtype;
         g->k = k;
         g->batch = batch;
         g->nchunk = nchunk;
-        g->ptr = reinterpret_cast<void* const*>(m);
-        g->len = reinterpret_cast<const size_t*>(m + o_len);
-        g->first = reinterpret_cast<const unsigned*>(m + o_first);
-        g->chunk_array = reinterpret_cast<const int*>(m + o_chunk);
+        g->chunks = static_cast<const GroupChunk*>(g->mem);
         *out = g;
         return TRAMP_OK;
     } catch (const std::bad_alloc&) {
@@ -240,12 +279,13 @@ static int group_run(tramp_ctx* ctx, const tramp_group* g, const tramp_group* pr
     int rc = tramp_ws_reserve(ctx, g->batch * (size_t)P * sizeof(double));
     if (rc) return rc;
     dim3 grid((unsigned)P, (unsigned)g->batch);
-    hipLaunchKernelGGL((group_squares_kernel<T, STEP>), grid, dim3(kBlock), 0, ctx->stream, dev_of(g), STEP ? prev->ptr : nullptr, ctx->ws);
+    hipLaunchKernelGGL((group_squares_kernel<T, STEP>), grid, dim3(kBlock), 0, ctx->stream, (unsigned)g->nchunk, g->chunks,
+                       STEP ? prev->chunks : nullptr, ctx->ws);
     if (!out)
         hipLaunchKernelGGL(group_norm_kernel, dim3((unsigned)g->batch), dim3(kBlock), 0, ctx->stream, ctx->ws, P, norm_d);
     else
-        hipLaunchKernelGGL((group_apply_kernel<T, STEP>), grid, dim3(kBlock), 0, ctx->stream, dev_of(g), STEP ? prev->ptr : nullptr, out->ptr,
-                           refresh, bound, ctx->ws, P, n_a, g->batch, a, a_prev, norm_d);
+        hipLaunchKernelGGL((group_apply_kernel<T, STEP>), grid, dim3(kBlock), 0, ctx->stream, (unsigned)g->nchunk, g->chunks,
+                           STEP ? prev->chunks : nullptr, out->chunks, refresh, bound, ctx->ws, P, n_a, g->batch, a, a_prev, norm_d);
     TRAMP_LAUNCH_CHECK(ctx);
     return TRAMP_OK;
 }
