@@ -24,7 +24,10 @@
 #include <new>
 #include <vector>
 
-struct LkItem;
+struct LkItem {
+    int token, start, end, slot;      // positions perm[start .. end); slot: of the partial sum, or the index of the heavy run
+};
+
 struct tramp_lookup {
     int device;
     int dtype;
@@ -36,17 +39,23 @@ struct tramp_lookup {
     const int* perm;             // [T]     positions sorted by token, ascending within a token, the padded ones last
     const int* off;              // [V + 1] the run of token v is perm[off[v] .. off[v + 1])
     const double* cnt;           // [2, K]  distinct counts and how many rows have them
+    const LkItem* chunks;        // heavy runs in chunks, one partial sum each
+    const LkItem* joins;         // {token, first chunk, one behind the last, index}
+    const LkItem* spreads;       // the chunks' positions and the padded ones
+    const LkItem* runs;          // runs for one workgroup
+    const int* waves;            // tokens of the runs for one wave
+    const int* light;            // tokens of the shorter runs, those of one position last
+    const int* idx;              // [V] place among the runs of two and more positions (short rows only)
+    const int* code;             // [T] that place, -1 where padded, -2 - token where the run is this position (short rows only)
     int K;
-    const LkItem* items;         // runs for whole workgroups (lookup_rows_kernel)
-    const LkItem* joins;         // heavy runs
-    const LkItem* spreads;       // their positions and the padded ones, in chunks
-    const int* waves;
-    unsigned n_items, n_joins, n_spreads, n_waves, n_slots;
+    unsigned n_chunks, n_joins, n_spreads, n_runs, n_waves, n_light, n_light2, n_multi;
     int lw;                      // log2 of the lanes per row
     unsigned tiles;              // column tiles per row
+    int row;                     // LK_TAIL / LK_WHOLE / LK_LINES
+    bool by_position;            // the message to x in the order of the positions
 };
 
-// what the kernels need of one instance, written by lookup_scalars_kernel
+// what the kernels need of one instance, written by lk_scalars
 struct LkScal {
     double az, ax, an, lik1;     // floored az, ax, a' before damping, ax scale^2
 };
@@ -54,14 +63,25 @@ struct LkScal {
 // ---------------------------------------------------------------- scalars
 // v, a' and n_eff of every instance from the table of distinct counts (n of them sum to at least n(n-1)/2 positions: 1414
 // at 10^6 positions), one workgroup per instance.
-__global__ __launch_bounds__(kBlock) void lookup_scalars_kernel(int K, const double* __restrict__ cnt, double V, double T,
-                                                                double padded, double s, int dir, const double* az_d,
-                                                                const double* ax_d, double damping, const double* a_old,
-                                                                LkScal* __restrict__ scal, double* v_out, double* a_new_out,
-                                                                double* n_eff_out) {
+struct LkScalArgs {
+    const double* cnt;
+    const double* az;
+    const double* ax;
+    const double* a_old;
+    LkScal* scal;
+    double* v_out;
+    double* a_new_out;
+    double* n_eff_out;
+    double V, T, padded, s, damping;
+    int K, dir;
+};
+
+__device__ void lk_scalars(const LkScalArgs& q, size_t b) {
     __shared__ double smem[kBlock / kWave];
-    const size_t b = blockIdx.x;
-    const double ax = ax_d[b], az = dir == TRAMP_BWD ? fmax(1e-11, az_d[b]) : az_d[b];     // linear_channel.py:92-94
+    const int K = q.K, dir = q.dir;
+    const double* cnt = q.cnt;
+    const double s = q.s;
+    const double ax = q.ax[b], az = dir == TRAMP_BWD ? fmax(1e-11, q.az[b]) : q.az[b];     // linear_channel.py:92-94
     const double lik1 = ax * s * s;
     double sv = 0.0, sn = 0.0, se = 0.0;
     for (int k = threadIdx.x; k < K; k += kBlock) {
@@ -83,20 +103,22 @@ __global__ __launch_bounds__(kBlock) void lookup_scalars_kernel(int K, const dou
     if (threadIdx.x != 0) return;
     double v, an;
     if (dir == TRAMP_BWD) {
-        v = sv / V;
-        an = (sn / V) / v;
+        v = sv / q.V;
+        an = (sn / q.V) / v;
     } else {
-        v = s * s * sv / T;
-        an = ((padded + sn) / T) / v;
+        v = s * s * sv / q.T;
+        an = ((q.padded + sn) / q.T) / v;
     }
     if (v > 1.7976931348623157e308) an = 0.0;                    // both precisions zero: 1 / v - a <= 0
     if (an < tmath::kAMin) an = tmath::kAMin;                    // (comparisons: a NaN passes through, tramp/base.py:252)
     if (an > tmath::kAMax) an = tmath::kAMax;
-    if (scal) scal[b] = LkScal{az, ax, an, lik1};
-    if (v_out) v_out[b] = v;
-    if (n_eff_out) n_eff_out[b] = se / V;
-    if (a_new_out) a_new_out[b] = damping != 0.0 ? damping * a_old[b] + (1.0 - damping) * an : an;
+    if (q.scal) q.scal[b] = LkScal{az, ax, an, lik1};
+    if (q.v_out) q.v_out[b] = v;
+    if (q.n_eff_out) q.n_eff_out[b] = se / q.V;
+    if (q.a_new_out) q.a_new_out[b] = q.damping != 0.0 ? q.damping * q.a_old[b] + (1.0 - q.damping) * an : an;
 }
+
+__global__ __launch_bounds__(kBlock) void lookup_scalars_kernel(LkScalArgs q) { lk_scalars(q, blockIdx.x); }
 
 // ---------------------------------------------------------------- rows in 16-byte pieces
 // A row of D elements is walked by LPR = min(64, 2^ceil(log2(D / N))) lanes, one 16-byte piece (N elements) per lane, in
@@ -112,11 +134,16 @@ template <> struct LkVec<double> {
     static constexpr int N = 2;
 };
 
-template <typename T, bool TAIL>
+// kinds of rows: LK_TAIL the last piece of a row is short; LK_WHOLE whole pieces; LK_LINES whole 128-byte lines, which nobody
+// else touches: read and written past the caches where they are used once
+enum { LK_TAIL = 0, LK_WHOLE = 1, LK_LINES = 2 };
+
+template <typename T, int ROW, bool ONCE = false>
 __device__ __forceinline__ void lk_load(const T* __restrict__ p, int valid, T (&v)[LkVec<T>::N]) {
     constexpr int N = LkVec<T>::N;
-    if (!TAIL || valid == N) {
-        const typename LkVec<T>::U u = *reinterpret_cast<const typename LkVec<T>::U*>(p);
+    using U = typename LkVec<T>::U;
+    if (ROW != LK_TAIL || valid == N) {
+        const U u = ROW == LK_LINES && ONCE ? __builtin_nontemporal_load(reinterpret_cast<const U*>(p)) : *reinterpret_cast<const U*>(p);
 #pragma unroll
         for (int i = 0; i < N; ++i) v[i] = u[i];
     } else {
@@ -125,14 +152,18 @@ __device__ __forceinline__ void lk_load(const T* __restrict__ p, int valid, T (&
     }
 }
 
-template <typename T, bool TAIL>
+template <typename T, int ROW>
 __device__ __forceinline__ void lk_store(T* p, int valid, const T (&v)[LkVec<T>::N]) {
     constexpr int N = LkVec<T>::N;
-    if (!TAIL || valid == N) {
-        typename LkVec<T>::U u;
+    using U = typename LkVec<T>::U;
+    if (ROW != LK_TAIL || valid == N) {
+        U u;
 #pragma unroll
         for (int i = 0; i < N; ++i) u[i] = v[i];
-        *reinterpret_cast<typename LkVec<T>::U*>(p) = u;
+        if (ROW == LK_LINES)
+            __builtin_nontemporal_store(u, reinterpret_cast<U*>(p));
+        else
+            *reinterpret_cast<U*>(p) = u;
     } else {
 #pragma unroll
         for (int i = 0; i < N; ++i)
@@ -158,26 +189,50 @@ template <typename T> __device__ __forceinline__ LkLane lk_lane(int lw, unsigned
     return k;
 }
 
+// Which instance, which workgroup of it, which column tile.  Workgroups go to the eight XCDs in turn; with `spread` the grid is
+// one-dimensional and all workgroups of an instance get numbers of one residue modulo 8: its table and positions, read and
+// written in the order of the tokens, then meet in one L2 (4 MiB) instead of in eight.
+struct LkPlace {
+    size_t b;
+    unsigned blk, tile;
+    bool in;
+};
+__device__ __forceinline__ LkPlace lk_place(unsigned blocks, unsigned tiles, unsigned batch, int spread) {
+    LkPlace p;
+    unsigned id = blockIdx.x;
+    if (spread) {
+        const unsigned per = blocks * tiles, j = id >> 3, r = j / per;
+        p.b = (size_t)r * 8 + (id & 7);
+        id = j - r * per;
+    } else {
+        p.b = blockIdx.y;
+    }
+    p.in = p.b < batch;
+    p.blk = id / tiles;
+    p.tile = id - p.blk * tiles;
+    return p;
+}
+
 // ---------------------------------------------------------------- x = scale z[token]
 // Bound by the write of x (and the read of the distinct rows of z).  Four rows per group in flight.
-template <typename T, bool TAIL>
-__global__ __launch_bounds__(kBlock) void lookup_apply_kernel(size_t V, size_t D, size_t n_pos, double s, int lw, unsigned tiles,
-                                                              const int* __restrict__ tok, const T* __restrict__ z, T* __restrict__ x) {
+template <typename T, int ROW>
+__global__ __launch_bounds__(kBlock) void lookup_apply_kernel(size_t V, size_t D, size_t n_pos, double s, int lw, unsigned blocks,
+                                                              unsigned tiles, unsigned batch, int spread, const int* __restrict__ tok, const T* __restrict__ z, T* __restrict__ x) {
     constexpr int N = LkVec<T>::N, UR = 4;
-    const size_t b = blockIdx.y;
-    const unsigned blk = blockIdx.x / tiles, tile = blockIdx.x - blk * tiles;
-    const LkLane k = lk_lane<T>(lw, tile, D);
-    if (k.valid <= 0) return;
+    const LkPlace w = lk_place(blocks, tiles, batch, spread);
+    const size_t b = w.b;
+    const LkLane k = lk_lane<T>(lw, w.tile, D);
+    if (!w.in || k.valid <= 0) return;
     const size_t G = kBlock >> lw;
     int row[UR];
     T v[UR][N];
-    size_t t0 = (size_t)blk * UR * G + k.group;
+    const size_t t0 = (size_t)w.blk * UR * G + k.group;
 #pragma unroll
     for (int i = 0; i < UR; ++i) row[i] = t0 + i * G < n_pos ? tok[t0 + i * G] : -1;
 #pragma unroll
     for (int i = 0; i < UR; ++i) {
         if (row[i] >= 0) {
-            lk_load<T, TAIL>(z + (b * V + (size_t)row[i]) * D + k.col, k.valid, v[i]);
+            lk_load<T, ROW>(z + (b * V + (size_t)row[i]) * D + k.col, k.valid, v[i]);
 #pragma unroll
             for (int e = 0; e < N; ++e) v[i][e] = T(s * (double)v[i][e]);
         } else {
@@ -187,16 +242,18 @@ __global__ __launch_bounds__(kBlock) void lookup_apply_kernel(size_t V, size_t D
     }
 #pragma unroll
     for (int i = 0; i < UR; ++i)
-        if (t0 + i * G < n_pos) lk_store<T, TAIL>(x + (b * n_pos + t0 + i * G) * D + k.col, k.valid, v[i]);
+        if (t0 + i * G < n_pos) lk_store<T, ROW>(x + (b * n_pos + t0 + i * G) * D + k.col, k.valid, v[i]);
 }
 
 // one column: N positions per lane, written as one piece
 template <typename T>
-__global__ __launch_bounds__(kBlock) void lookup_apply1_kernel(size_t V, size_t n_pos, double s, const int* __restrict__ tok,
+__global__ __launch_bounds__(kBlock) void lookup_apply1_kernel(size_t V, size_t n_pos, double s, unsigned blocks, unsigned batch, int spread,
+                                                               const int* __restrict__ tok,
                                                                const T* __restrict__ z, T* __restrict__ x) {
     constexpr int N = LkVec<T>::N;
-    const size_t b = blockIdx.y, t = ((size_t)blockIdx.x * kBlock + threadIdx.x) * N;
-    if (t >= n_pos) return;
+    const LkPlace w = lk_place(blocks, 1, batch, spread);
+    const size_t b = w.b, t = ((size_t)w.blk * kBlock + threadIdx.x) * N;
+    if (!w.in || t >= n_pos) return;
     const int valid = n_pos - t >= N ? N : (int)(n_pos - t);
     int row[N];
     T v[N];
@@ -204,7 +261,7 @@ __global__ __launch_bounds__(kBlock) void lookup_apply1_kernel(size_t V, size_t 
     for (int i = 0; i < N; ++i) row[i] = i < valid ? tok[t + i] : -1;
 #pragma unroll
     for (int i = 0; i < N; ++i) v[i] = row[i] >= 0 ? T(s * (double)z[b * V + (size_t)row[i]]) : T(0);
-    lk_store<T, true>(x + b * n_pos + t, valid, v);
+    lk_store<T, LK_TAIL>(x + b * n_pos + t, valid, v);
 }
 
 // ---------------------------------------------------------------- sums over the runs
@@ -212,30 +269,34 @@ __global__ __launch_bounds__(kBlock) void lookup_apply1_kernel(size_t V, size_t 
 //   light  run <= kKeep                       one group, all rows of the run in flight at once
 //   wave   run <= kKeep * 64 / LPR            the groups of one wave, joined by a butterfly
 //   block  run <= kKeep * 256 / LPR           the groups of one workgroup, the four waves joined through LDS
-//   heavy  longer                             chunks of a multiple of that; partial sums in double, joined by a second launch
+//   heavy  longer                             chunks of a multiple of that, summed in a first launch (lookup_chunks_kernel),
+//                                             the partial sums in double joined by one workgroup in the second
 // In the first three every row stays in registers from the sum to the message that goes back to its position: the message to
-// the positions reads bx once.  Only the runs of the last kind read it twice.
-constexpr int kKeep = 16;
-
-struct LkItem {
-    int token, start, end, slot;      // slot: of the partial sum; < 0: the item is a whole run
-};
+// the positions reads bx once.  Only the heavy runs are read twice, the second time in a third launch.
+// kKeep: 8 rows in flight per group leave 5 to 8 waves per SIMD; 16 leave 3 to 5 and cost a third (gradient 121 against 84 us,
+// message to 10^6 positions of 64 columns 136 against 104 us), 4 make longer runs of every kind (89 and 103 us).
+constexpr int kKeep = 8;
 
 struct LkArgs {
     const int* off;
     const int* perm;
-    const LkItem* items;         // [n_items] heavy chunks, then the block runs
-    const int* waves;            // [n_waves] tokens of the wave runs
+    const LkItem* chunks;
+    const LkItem* joins;
+    const LkItem* runs;
+    const int* waves;
+    const int* light;            // null: all rows of the table (those of the kinds above left out)
+    const int* idx;
     size_t V, D, T;
-    unsigned n_items, n_waves, wave_blocks, blocks, tiles, n_slots;
-    int lw;
+    unsigned n_chunks, n_joins, n_runs, n_waves, wave_blocks, n_light, n_multi, blocks, tiles, batch;
+    int lw, spread;
     double s;
 };
 
-enum { LK_GRAD = 0, LK_BWD = 1, LK_FWD = 2 };
+// what is made of the sum of a run: the gradient, the message to the table, the message to its positions, scale times the mean
+enum { LK_GRAD = 0, LK_BWD = 1, LK_FWD = 2, LK_MEAN = 3 };
 
 // rows perm[j0 + sub], perm[j0 + sub + S], ... of the run [j0, j0 + c), S = 1 << ls: added into acc, kept if KEEP (c <= kKeep S)
-template <typename T, bool TAIL, bool KEEP>
+template <typename T, int ROW, bool KEEP, bool ONCE>
 __device__ __forceinline__ void lk_gather(const LkArgs& a, const T* __restrict__ xb, const LkLane& k, int j0, int c, int sub, int ls,
                                           double (&acc)[LkVec<T>::N], int (&pj)[kKeep], T (&rows)[kKeep][LkVec<T>::N]) {
     constexpr int N = LkVec<T>::N;
@@ -253,7 +314,7 @@ __device__ __forceinline__ void lk_gather(const LkArgs& a, const T* __restrict__
             if (base + q < cnt) {
 #pragma unroll
                 for (int i = q; i < q + 4; ++i)
-                    if (base + i < cnt) lk_load<T, TAIL>(xb + (size_t)pj[i] * a.D + k.col, k.valid, rows[i]);
+                    if (base + i < cnt) lk_load<T, ROW, ONCE>(xb + (size_t)pj[i] * a.D + k.col, k.valid, rows[i]);
             }
 #pragma unroll
         for (int i = 0; i < kKeep; ++i)
@@ -284,8 +345,20 @@ template <int N> __device__ __forceinline__ void lk_block_join(const LkLane& k, 
     for (int e = 0; e < N; ++e) acc[e] = ((sm[0][lane][e] + sm[1][lane][e]) + sm[2][lane][e]) + sm[3][lane][e];
 }
 
-// what is done with the sum of row v: the gradient or the message to the table; `first`: one group of those that hold the sum
-template <typename T, bool TAIL, int MODE>
+// scale times the posterior mean of a row with the sum acc
+template <typename T, int ROW>
+__device__ __forceinline__ void lk_mean(const LkArgs& a, const LkScal& c, const LkLane& k, size_t b, int v, int count, const T* __restrict__ bz,
+                                        const double (&acc)[LkVec<T>::N], double (&sr)[LkVec<T>::N]) {
+    constexpr int N = LkVec<T>::N;
+    T z[N];
+    lk_load<T, ROW>(bz + (b * a.V + (size_t)v) * a.D + k.col, k.valid, z);
+    const double prec = c.az + c.lik1 * (double)count;
+#pragma unroll
+    for (int e = 0; e < N; ++e) sr[e] = a.s * (((double)z[e] + a.s * acc[e]) / prec);
+}
+
+// the gradient or the message to the table
+template <typename T, int ROW, int MODE>
 __device__ __forceinline__ void lk_row_out(const LkArgs& a, const LkScal& c, const LkLane& k, size_t b, int v, int count,
                                            const double (&acc)[LkVec<T>::N], const T* __restrict__ bz, double damping, const T* b_old,
                                            T* out, T* __restrict__ r_out) {
@@ -298,8 +371,8 @@ __device__ __forceinline__ void lk_row_out(const LkArgs& a, const LkScal& c, con
     } else {
         const double lik = c.lik1 * (double)count, prec = c.az + lik;
         T z[N], r[N], old[N];
-        lk_load<T, TAIL>(bz + at, k.valid, z);
-        if (damping != 0.0) lk_load<T, TAIL>(b_old + at, k.valid, old);
+        lk_load<T, ROW, true>(bz + at, k.valid, z);
+        if (damping != 0.0) lk_load<T, ROW>(b_old + at, k.valid, old);
 #pragma unroll
         for (int e = 0; e < N; ++e) {
             const double g = a.s * acc[e];
@@ -308,43 +381,74 @@ __device__ __forceinline__ void lk_row_out(const LkArgs& a, const LkScal& c, con
             o[e] = T(m);
             r[e] = T(((double)z[e] + g) / prec);
         }
-        if (r_out) lk_store<T, TAIL>(r_out + at, k.valid, r);
+        if (r_out) lk_store<T, ROW>(r_out + at, k.valid, r);
     }
-    lk_store<T, TAIL>(out + at, k.valid, o);
+    lk_store<T, ROW>(out + at, k.valid, o);
 }
 
-// the message to one position of a row with posterior mean r: rx = s r, b' = rx (ax + a') - bx
-template <typename T, bool TAIL>
-__device__ __forceinline__ void lk_position_out(const LkArgs& a, double asum, const LkLane& k, size_t b, int t,
+// the message to one position: b' = rx (ax + a') - bx with rx = scale r
+template <typename T, int ROW>
+__device__ __forceinline__ void lk_position_out(const LkArgs& a, double asum, const LkLane& k, size_t b, size_t t,
                                                 const double (&sr)[LkVec<T>::N], const T (&bx)[LkVec<T>::N], double damping, const T* b_old,
                                                 T* out, T* __restrict__ r_out) {
     constexpr int N = LkVec<T>::N;
-    const size_t at = (b * a.T + (size_t)t) * a.D + k.col;
+    const size_t at = (b * a.T + t) * a.D + k.col;
     T o[N], old[N];
-    if (damping != 0.0) lk_load<T, TAIL>(b_old + at, k.valid, old);
+    if (damping != 0.0) lk_load<T, ROW>(b_old + at, k.valid, old);
 #pragma unroll
     for (int e = 0; e < N; ++e) {
         double m = sr[e] * asum - (double)bx[e];
         if (damping != 0.0) m = damping * (double)old[e] + (1.0 - damping) * m;
         o[e] = T(m);
     }
-    lk_store<T, TAIL>(out + at, k.valid, o);
+    lk_store<T, ROW>(out + at, k.valid, o);
     if (r_out) {
 #pragma unroll
         for (int e = 0; e < N; ++e) o[e] = T(sr[e]);
-        lk_store<T, TAIL>(r_out + at, k.valid, o);
+        lk_store<T, ROW>(r_out + at, k.valid, o);
     }
 }
 
-template <typename T, bool TAIL, int MODE>
-__global__ __launch_bounds__(kBlock) void lookup_rows_kernel(LkArgs a, const LkScal* __restrict__ scal, const T* __restrict__ bz,
-                                                             const T* __restrict__ x, double damping, const T* b_old, T* out,
-                                                             T* __restrict__ r_out, double* __restrict__ partials) {
+// First launch: the partial sums of the heavy runs; one more workgroup per instance makes its scalars.
+template <typename T, int ROW, bool ONCE>
+__global__ __launch_bounds__(kBlock) void lookup_chunks_kernel(LkArgs a, LkScalArgs q, const T* __restrict__ x, double* __restrict__ partials) {
     constexpr int N = LkVec<T>::N;
     __shared__ double sm[kBlock / kWave][kWave][N];
     const size_t b = blockIdx.y;
-    const unsigned blk = blockIdx.x / a.tiles, tile = blockIdx.x - blk * a.tiles;
-    const LkLane k = lk_lane<T>(a.lw, tile, a.D);
+    if (blockIdx.x == a.n_chunks * a.tiles) {
+        lk_scalars(q, b);
+        return;
+    }
+    const unsigned blk = blockIdx.x / a.tiles;
+    const LkLane k = lk_lane<T>(a.lw, blockIdx.x - blk * a.tiles, a.D);
+    const LkItem it = a.chunks[blk];
+    double acc[N];
+    int pj[kKeep];
+    T rows[kKeep][N];
+#pragma unroll
+    for (int e = 0; e < N; ++e) acc[e] = 0.0;
+    if (k.valid > 0) lk_gather<T, ROW, false, ONCE>(a, x + b * a.T * a.D, k, it.start, it.end - it.start, k.group, 8 - a.lw, acc, pj, rows);
+    lk_block_join<N>(k, acc, sm);
+    if (threadIdx.x >= (1u << a.lw) || k.valid <= 0) return;
+    double* p = partials + (b * a.n_chunks + (size_t)it.slot) * a.D + k.col;
+#pragma unroll
+    for (int e = 0; e < N; ++e)
+        if (e < k.valid) p[e] = acc[e];
+}
+
+// Second launch: every run.  Workgroups, in this order: joins of the partial sums, block runs, wave runs, light ones.
+template <typename T, int ROW, int MODE>
+__global__ __launch_bounds__(kBlock) void lookup_rows_kernel(LkArgs a, const LkScal* __restrict__ scal, const T* __restrict__ bz,
+                                                             const T* __restrict__ x, double damping, const T* b_old, T* out,
+                                                             T* __restrict__ r_out, const double* __restrict__ partials,
+                                                             double* __restrict__ sr_ws) {
+    constexpr int N = LkVec<T>::N;
+    __shared__ double sm[kBlock / kWave][kWave][N];
+    const LkPlace place = lk_place(a.blocks, a.tiles, a.batch, a.spread);
+    if (!place.in) return;
+    const size_t b = place.b;
+    unsigned blk = place.blk;
+    const LkLane k = lk_lane<T>(a.lw, place.tile, a.D);
     LkScal c{};
     if (MODE != LK_GRAD) c = scal[b];
     const T* xb = x + b * a.T * a.D;
@@ -354,126 +458,92 @@ __global__ __launch_bounds__(kBlock) void lookup_rows_kernel(LkArgs a, const LkS
     T rows[kKeep][N];
 #pragma unroll
     for (int e = 0; e < N; ++e) acc[e] = 0.0;
-    int v, j0, run, count, sub, ls;
+    int v, j0, count, sub, ls, place_ws = -1;
     bool first = true;
-    if (blk < a.n_items) {
-        // a block run, or a chunk of a heavy one
-        const LkItem it = a.items[blk];
+    if (blk < a.n_joins) {
+        const LkItem it = a.joins[blk];
+        v = it.token;
+        count = a.off[v + 1] - a.off[v];
+        const int G = kBlock >> a.lw;
+        const double* p = partials + b * a.n_chunks * a.D + k.col;
+#pragma unroll 4
+        for (int j = it.start + k.group; j < it.end; j += G) {
+#pragma unroll
+            for (int e = 0; e < N; ++e) acc[e] += e < k.valid ? p[(size_t)j * a.D + e] : 0.0;
+        }
+        lk_block_join<N>(k, acc, sm);
+        first = threadIdx.x < (1u << a.lw);
+        place_ws = it.slot;
+        sub = ls = j0 = 0;
+    } else if ((blk -= a.n_joins) < a.n_runs) {
+        const LkItem it = a.runs[blk];
         v = it.token;
         j0 = it.start;
-        run = it.end - it.start;
+        count = it.end - it.start;
         sub = k.group;
         ls = 8 - a.lw;
-        first = threadIdx.x < (1 << a.lw);
-        if (it.slot >= 0) {
-            if (act) lk_gather<T, TAIL, false>(a, xb, k, j0, run, sub, ls, acc, pj, rows);
-            lk_block_join<N>(k, acc, sm);
-            if (first && act) {
-                double* p = partials + (b * a.n_slots + (size_t)it.slot) * a.D + k.col;
-#pragma unroll
-                for (int e = 0; e < N; ++e)
-                    if (e < k.valid) p[e] = acc[e];
-            }
-            return;
-        }
-        if (act) lk_gather<T, TAIL, true>(a, xb, k, j0, run, sub, ls, acc, pj, rows);
+        first = threadIdx.x < (1u << a.lw);
+        if (act) lk_gather<T, ROW, true, true>(a, xb, k, j0, count, sub, ls, acc, pj, rows);
         lk_block_join<N>(k, acc, sm);
-        count = run;
     } else {
-        if (blk < a.n_items + a.wave_blocks) {
-            const unsigned w = (blk - a.n_items) * (kBlock / kWave) + (threadIdx.x >> 6);
+        blk -= a.n_runs;
+        if (blk < a.wave_blocks) {
+            const unsigned w = blk * (kBlock / kWave) + (threadIdx.x >> 6);
             if (w >= a.n_waves) return;
             v = a.waves[w];
             sub = (threadIdx.x & 63) >> a.lw;
             ls = 6 - a.lw;
-            first = (threadIdx.x & 63) < (1 << a.lw);
+            first = (threadIdx.x & 63) < (1u << a.lw);
         } else {
-            const size_t u = (size_t)(blk - a.n_items - a.wave_blocks) * (kBlock >> a.lw) + k.group;
-            if (u >= a.V) return;
-            v = (int)u;
+            const size_t u = (size_t)(blk - a.wave_blocks) * (kBlock >> a.lw) + k.group;
+            if (u >= a.n_light) return;
+            v = a.light ? a.light[u] : (int)u;
             sub = 0;
             ls = 0;
         }
         j0 = a.off[v];
-        run = count = a.off[v + 1] - j0;
-        if (ls == 0 && run > kKeep) return;                        // listed above
-        if (act) lk_gather<T, TAIL, true>(a, xb, k, j0, run, sub, ls, acc, pj, rows);
+        count = a.off[v + 1] - j0;
+        if (ls == 0 && count > kKeep) return;                      // of another kind
+        if (act) lk_gather<T, ROW, true, true>(a, xb, k, j0, count, sub, ls, acc, pj, rows);
         if (ls) lk_wave_join<N>(a.lw, acc);
     }
     if (!act) return;
-    if (MODE != LK_FWD) {
-        if (first) lk_row_out<T, TAIL, MODE>(a, c, k, b, v, count, acc, bz, damping, b_old, out, r_out);
+    if (MODE == LK_GRAD || MODE == LK_BWD) {
+        if (first) lk_row_out<T, ROW, MODE>(a, c, k, b, v, count, acc, bz, damping, b_old, out, r_out);
         return;
     }
-    if (count == 0) return;
-    T z[N];
-    lk_load<T, TAIL>(bz + (b * a.V + (size_t)v) * a.D + k.col, k.valid, z);
-    const double prec = c.az + c.lik1 * (double)count, asum = c.ax + c.an;
     double sr[N];
+    lk_mean<T, ROW>(a, c, k, b, v, count, bz, acc, sr);
+    if (MODE == LK_MEAN || place_ws >= 0) {
+        if (!first) return;
+        double* r = sr_ws + (MODE == LK_MEAN ? b * a.n_multi + (size_t)a.idx[v] : b * a.n_joins + (size_t)place_ws) * a.D + k.col;
 #pragma unroll
-    for (int e = 0; e < N; ++e) sr[e] = a.s * (((double)z[e] + a.s * acc[e]) / prec);
-    const int cnt = run > sub ? ((run - sub - 1) >> ls) + 1 : 0;
+        for (int e = 0; e < N; ++e)
+            if (e < k.valid) r[e] = sr[e];
+        return;
+    }
+    const int cnt = count > sub ? ((count - sub - 1) >> ls) + 1 : 0;
 #pragma unroll
     for (int i = 0; i < kKeep; ++i)
-        if (i < cnt) lk_position_out<T, TAIL>(a, asum, k, b, pj[i], sr, rows[i], damping, b_old, out, r_out);
+        if (i < cnt) lk_position_out<T, ROW>(a, c.ax + c.an, k, b, (size_t)pj[i], sr, rows[i], damping, b_old, out, r_out);
 }
 
-// the partial sums of a heavy run: {token, first slot, one behind the last, index among the heavy runs}
-template <typename T, bool TAIL, int MODE>
-__global__ __launch_bounds__(kBlock) void lookup_join_kernel(LkArgs a, const LkItem* __restrict__ joins, unsigned n_joins,
-                                                             const LkScal* __restrict__ scal, const T* __restrict__ bz,
-                                                             const double* __restrict__ partials, double damping, const T* b_old, T* out,
-                                                             T* __restrict__ r_out, double* __restrict__ r_ws) {
-    constexpr int N = LkVec<T>::N;
-    __shared__ double sm[kBlock / kWave][kWave][N];
-    const size_t b = blockIdx.y;
-    const unsigned blk = blockIdx.x / a.tiles, tile = blockIdx.x - blk * a.tiles;
-    const LkLane k = lk_lane<T>(a.lw, tile, a.D);
-    LkScal c{};
-    if (MODE != LK_GRAD) c = scal[b];
-    const LkItem it = joins[blk];
-    const int v = it.token, G = kBlock >> a.lw, count = a.off[v + 1] - a.off[v];
-    double acc[N];
-#pragma unroll
-    for (int e = 0; e < N; ++e) acc[e] = 0.0;
-    const double* p = partials + b * a.n_slots * a.D + k.col;
-#pragma unroll 4
-    for (int j = it.start + k.group; j < it.end; j += G) {
-#pragma unroll
-        for (int e = 0; e < N; ++e) acc[e] += e < k.valid ? p[(size_t)j * a.D + e] : 0.0;
-    }
-    lk_block_join<N>(k, acc, sm);
-    if (threadIdx.x >= (1u << a.lw) || k.valid <= 0) return;
-    if (MODE != LK_FWD) {
-        lk_row_out<T, TAIL, MODE>(a, c, k, b, v, count, acc, bz, damping, b_old, out, r_out);
-        return;
-    }
-    T z[N];
-    lk_load<T, TAIL>(bz + (b * a.V + (size_t)v) * a.D + k.col, k.valid, z);
-    const double prec = c.az + c.lik1 * (double)count;
-    double* r = r_ws + (b * n_joins + (size_t)it.slot) * a.D + k.col;
-#pragma unroll
-    for (int e = 0; e < N; ++e)
-        if (e < k.valid) r[e] = a.s * (((double)z[e] + a.s * acc[e]) / prec);
-}
-
-// the message to the positions of the heavy runs and to the padded ones: {-, start, end, index of the heavy run or -1}
-template <typename T, bool TAIL>
-__global__ __launch_bounds__(kBlock) void lookup_spread_kernel(LkArgs a, const LkItem* __restrict__ spreads, unsigned n_joins,
-                                                               const LkScal* __restrict__ scal, const double* __restrict__ r_ws,
-                                                               const T* __restrict__ bx, double damping, const T* b_old, T* out,
-                                                               T* __restrict__ r_out) {
+// Third launch of the message to the positions: those of the heavy runs and the padded ones (slot -1: rx = 0)
+template <typename T, int ROW>
+__global__ __launch_bounds__(kBlock) void lookup_spread_kernel(LkArgs a, const LkItem* __restrict__ spreads, const LkScal* __restrict__ scal,
+                                                               const double* __restrict__ sr_ws, const T* __restrict__ bx, double damping,
+                                                               const T* b_old, T* out, T* __restrict__ r_out) {
     constexpr int N = LkVec<T>::N, UR = 4;
     const size_t b = blockIdx.y;
-    const unsigned blk = blockIdx.x / a.tiles, tile = blockIdx.x - blk * a.tiles;
-    const LkLane k = lk_lane<T>(a.lw, tile, a.D);
+    const unsigned blk = blockIdx.x / a.tiles;
+    const LkLane k = lk_lane<T>(a.lw, blockIdx.x - blk * a.tiles, a.D);
     if (k.valid <= 0) return;
     const LkItem it = spreads[blk];
     const double asum = scal[b].ax + scal[b].an;
     double sr[N];
 #pragma unroll
     for (int e = 0; e < N; ++e)
-        sr[e] = it.slot >= 0 && e < k.valid ? r_ws[(b * n_joins + (size_t)it.slot) * a.D + k.col + e] : 0.0;
+        sr[e] = it.slot >= 0 && e < k.valid ? sr_ws[(b * a.n_joins + (size_t)it.slot) * a.D + k.col + e] : 0.0;
     const int G = kBlock >> a.lw;
     for (int j = it.start + k.group; j < it.end; j += UR * G) {
         int t[UR];
@@ -482,10 +552,94 @@ __global__ __launch_bounds__(kBlock) void lookup_spread_kernel(LkArgs a, const L
         for (int i = 0; i < UR; ++i) t[i] = j + i * G < it.end ? a.perm[j + i * G] : -1;
 #pragma unroll
         for (int i = 0; i < UR; ++i)
-            if (t[i] >= 0) lk_load<T, TAIL>(bx + (b * a.T + (size_t)t[i]) * a.D + k.col, k.valid, v[i]);
+            if (t[i] >= 0) lk_load<T, ROW>(bx + (b * a.T + (size_t)t[i]) * a.D + k.col, k.valid, v[i]);
 #pragma unroll
         for (int i = 0; i < UR; ++i)
-            if (t[i] >= 0) lk_position_out<T, TAIL>(a, asum, k, b, t[i], sr, v[i], damping, b_old, out, r_out);
+            if (t[i] >= 0) lk_position_out<T, ROW>(a, asum, k, b, (size_t)t[i], sr, v[i], damping, b_old, out, r_out);
+    }
+}
+
+// ---------------------------------------------------------------- the message to x in the order of the positions
+// Rows shorter than half a line cost a line each when they are read or written in the order of the tokens.  Here the sums of the
+// runs of two and more positions leave scale r in double (LK_MEAN), and x is walked in its own order: a position that is
+// alone in its run has its sum at hand, the others fetch theirs.  One column: a lane takes one 16-byte piece of positions.
+template <typename T, int ROW>
+__global__ __launch_bounds__(kBlock) void lookup_positions_kernel(LkArgs a, const int* __restrict__ code, const LkScal* __restrict__ scal,
+                                                                  const T* __restrict__ bz, const double* __restrict__ sr_ws,
+                                                                  const T* __restrict__ bx, double damping, const T* b_old, T* out,
+                                                                  T* __restrict__ r_out) {
+    constexpr int N = LkVec<T>::N, UR = 4;
+    const LkPlace place = lk_place(a.blocks, a.tiles, a.batch, a.spread);
+    const size_t b = place.b;
+    const LkLane k = lk_lane<T>(a.lw, place.tile, a.D);
+    if (!place.in || k.valid <= 0) return;
+    const LkScal c = scal[b];
+    const double asum = c.ax + c.an, prec1 = c.az + c.lik1;
+    const size_t G = kBlock >> a.lw, t0 = (size_t)place.blk * UR * G + k.group;
+    int w[UR];
+    T v[UR][N], z[UR][N];
+    double sr[UR][N];
+#pragma unroll
+    for (int i = 0; i < UR; ++i) w[i] = t0 + i * G < a.T ? code[t0 + i * G] : -1;
+#pragma unroll
+    for (int i = 0; i < UR; ++i) {
+        if (t0 + i * G < a.T) lk_load<T, ROW>(bx + (b * a.T + t0 + i * G) * a.D + k.col, k.valid, v[i]);
+        if (w[i] <= -2) lk_load<T, ROW>(bz + (b * a.V + (size_t)(-2 - w[i])) * a.D + k.col, k.valid, z[i]);
+#pragma unroll
+        for (int e = 0; e < N; ++e)
+            sr[i][e] = w[i] >= 0 && e < k.valid ? sr_ws[(b * a.n_multi + (size_t)w[i]) * a.D + k.col + e] : 0.0;
+    }
+#pragma unroll
+    for (int i = 0; i < UR; ++i) {
+        if (w[i] <= -2) {
+#pragma unroll
+            for (int e = 0; e < N; ++e) sr[i][e] = a.s * (((double)z[i][e] + a.s * (double)v[i][e]) / prec1);
+        }
+        if (t0 + i * G < a.T) lk_position_out<T, ROW>(a, asum, k, b, t0 + i * G, sr[i], v[i], damping, b_old, out, r_out);
+    }
+}
+
+template <typename T>
+__global__ __launch_bounds__(kBlock) void lookup_positions1_kernel(LkArgs a, const int* __restrict__ code, const LkScal* __restrict__ scal,
+                                                                   const T* __restrict__ bz, const double* __restrict__ sr_ws,
+                                                                   const T* __restrict__ bx, double damping, const T* b_old, T* out,
+                                                                   T* __restrict__ r_out) {
+    constexpr int N = LkVec<T>::N;
+    const LkPlace place = lk_place(a.blocks, 1, a.batch, a.spread);
+    const size_t b = place.b, t = ((size_t)place.blk * kBlock + threadIdx.x) * N;
+    if (!place.in || t >= a.T) return;
+    const LkScal c = scal[b];
+    const double asum = c.ax + c.an, prec1 = c.az + c.lik1;
+    const int valid = a.T - t >= N ? N : (int)(a.T - t);
+    int w[N];
+    T v[N], o[N], old[N];
+    double z[N];
+    if (valid == N) {
+        typedef int I __attribute__((ext_vector_type(N), aligned(4)));
+        const I u = *reinterpret_cast<const I*>(code + t);
+#pragma unroll
+        for (int i = 0; i < N; ++i) w[i] = u[i];
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i) w[i] = i < valid ? code[t + i] : -1;
+    }
+    lk_load<T, LK_TAIL>(bx + b * a.T + t, valid, v);
+    if (damping != 0.0) lk_load<T, LK_TAIL>(b_old + b * a.T + t, valid, old);
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+        z[i] = w[i] >= 0 ? sr_ws[b * a.n_multi + (size_t)w[i]] : w[i] == -1 ? 0.0 : (double)bz[b * a.V + (size_t)(-2 - w[i])];
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        if (w[i] <= -2) z[i] = a.s * ((z[i] + a.s * (double)v[i]) / prec1);
+        double m = z[i] * asum - (double)v[i];
+        if (damping != 0.0) m = damping * (double)old[i] + (1.0 - damping) * m;
+        o[i] = T(m);
+    }
+    lk_store<T, LK_TAIL>(out + b * a.T + t, valid, o);
+    if (r_out) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) o[i] = T(z[i]);
+        lk_store<T, LK_TAIL>(r_out + b * a.T + t, valid, o);
     }
 }
 
@@ -546,22 +700,27 @@ extern "C" int tramp_lookup_create(tramp_ctx* ctx, int dtype, size_t n_rows, siz
             for (size_t t = 0; t < n_pos; ++t) perm[tokens_h[t] >= 0 ? (size_t)at[(size_t)tokens_h[t]]++ : pad++] = (int)t;
         }
         // lanes per row and the cut by run lengths (lookup_rows_kernel)
-        const size_t piece = 16 / dtype_size(dtype), pieces = (n_cols + piece - 1) / piece;
+        const size_t e = dtype_size(dtype), piece = 16 / e, pieces = (n_cols + piece - 1) / piece;
         int lw = 0;
         while (lw < 6 && ((size_t)1 << lw) < pieces) ++lw;
         const size_t tiles = (pieces + ((size_t)1 << lw) - 1) >> lw;
         const int per_wave = kKeep << (6 - lw), per_block = kKeep << (8 - lw);
+        const bool by_position = n_cols * e < 64;
         std::vector<LkItem> chunks, runs, joins, spreads;
-        std::vector<int> waves;
+        std::vector<int> waves, light, single, idx, code;
         for (size_t v = 0; v < n_rows; ++v) {
             const int c = counts[v], j0 = off[v];
-            if (c <= kKeep) continue;
-            if (c <= per_wave) {
+            if (c == 0) continue;
+            if (c == 1) {
+                single.push_back((int)v);
+            } else if (c <= kKeep) {
+                light.push_back((int)v);
+            } else if (c <= per_wave) {
                 waves.push_back((int)v);
             } else if (c <= per_block) {
                 runs.push_back(LkItem{(int)v, j0, j0 + c, -1});
             } else {
-                // at most 256 partial sums per run: the second launch adds them in one workgroup
+                // at most 256 partial sums per run: one workgroup adds them
                 const long step = (long)per_block * (((long)c + 256L * per_block - 1) / (256L * per_block));
                 const int slot0 = (int)chunks.size();
                 for (long j = 0; j < c; j += step) {
@@ -574,8 +733,19 @@ extern "C" int tramp_lookup_create(tramp_ctx* ctx, int dtype, size_t n_rows, siz
         }
         for (size_t j = seen; j < n_pos; j += (size_t)per_block)
             spreads.push_back(LkItem{-1, (int)j, (int)std::min(n_pos, j + (size_t)per_block), -1});
-        const size_t n_slots = chunks.size();
-        chunks.insert(chunks.end(), runs.begin(), runs.end());
+        const size_t n_light2 = light.size();
+        light.insert(light.end(), single.begin(), single.end());
+        size_t n_multi = 0;
+        if (by_position) {
+            idx.assign(n_rows, -1);
+            for (size_t v = 0; v < n_rows; ++v)
+                if (counts[v] > 1) idx[v] = (int)n_multi++;
+            code.resize(n_pos);
+            for (size_t t = 0; t < n_pos; ++t) {
+                const int v = tokens_h[t];
+                code[t] = v < 0 ? -1 : counts[(size_t)v] == 1 ? -2 - v : idx[(size_t)v];
+            }
+        }
         std::sort(counts.begin(), counts.end());
         std::vector<double> cval, cmul;
         for (size_t v = 0; v < n_rows; ++v) {
@@ -596,9 +766,10 @@ extern "C" int tramp_lookup_create(tramp_ctx* ctx, int dtype, size_t n_rows, siz
             return at;
         };
         const size_t o_tok = put(tokens_h, n_pos * 4), o_perm = put(perm.data(), n_pos * 4), o_off = put(off.data(), (n_rows + 1) * 4);
-        const size_t o_cnt = put(cval.data(), 2 * K * 8), o_items = put(chunks.data(), chunks.size() * sizeof(LkItem));
+        const size_t o_cnt = put(cval.data(), 2 * K * 8), o_chunks = put(chunks.data(), chunks.size() * sizeof(LkItem));
         const size_t o_joins = put(joins.data(), joins.size() * sizeof(LkItem)), o_spreads = put(spreads.data(), spreads.size() * sizeof(LkItem));
-        const size_t o_waves = put(waves.data(), waves.size() * 4);
+        const size_t o_runs = put(runs.data(), runs.size() * sizeof(LkItem)), o_waves = put(waves.data(), waves.size() * 4);
+        const size_t o_light = put(light.data(), light.size() * 4), o_idx = put(idx.data(), idx.size() * 4), o_code = put(code.data(), code.size() * 4);
         tramp_lookup* lk = new tramp_lookup();
         *lk = tramp_lookup{};
         (void)hipSetDevice(ctx->device);
@@ -608,12 +779,12 @@ extern "C" int tramp_lookup_create(tramp_ctx* ctx, int dtype, size_t n_rows, siz
             return tramp_fail(ctx, TRAMP_ENOMEM, "tramp_lookup_create", "hipMalloc failed");
         }
         char* m = static_cast<char*>(lk->mem);
-        hipError_t e = hipMemcpyAsync(m, host.data(), host.size(), hipMemcpyHostToDevice, ctx->stream);
-        if (e == hipSuccess) e = hipStreamSynchronize(ctx->stream);      // the host array ends here
-        if (e != hipSuccess) {
+        hipError_t err = hipMemcpyAsync(m, host.data(), host.size(), hipMemcpyHostToDevice, ctx->stream);
+        if (err == hipSuccess) err = hipStreamSynchronize(ctx->stream);  // the host array ends here
+        if (err != hipSuccess) {
             (void)hipFree(lk->mem);
             delete lk;
-            return tramp_fail(ctx, TRAMP_EHIP, "tramp_lookup_create", hipGetErrorString(e));
+            return tramp_fail(ctx, TRAMP_EHIP, "tramp_lookup_create", hipGetErrorString(err));
         }
         lk->device = ctx->device;
         lk->dtype = dtype;
@@ -626,18 +797,27 @@ extern "C" int tramp_lookup_create(tramp_ctx* ctx, int dtype, size_t n_rows, siz
         lk->perm = reinterpret_cast<const int*>(m + o_perm);
         lk->off = reinterpret_cast<const int*>(m + o_off);
         lk->cnt = reinterpret_cast<const double*>(m + o_cnt);
-        lk->K = (int)K;
-        lk->items = reinterpret_cast<const LkItem*>(m + o_items);
+        lk->chunks = reinterpret_cast<const LkItem*>(m + o_chunks);
         lk->joins = reinterpret_cast<const LkItem*>(m + o_joins);
         lk->spreads = reinterpret_cast<const LkItem*>(m + o_spreads);
+        lk->runs = reinterpret_cast<const LkItem*>(m + o_runs);
         lk->waves = reinterpret_cast<const int*>(m + o_waves);
-        lk->n_items = (unsigned)chunks.size();
+        lk->light = reinterpret_cast<const int*>(m + o_light);
+        lk->idx = reinterpret_cast<const int*>(m + o_idx);
+        lk->code = reinterpret_cast<const int*>(m + o_code);
+        lk->K = (int)K;
+        lk->n_chunks = (unsigned)chunks.size();
         lk->n_joins = (unsigned)joins.size();
         lk->n_spreads = (unsigned)spreads.size();
+        lk->n_runs = (unsigned)runs.size();
         lk->n_waves = (unsigned)waves.size();
-        lk->n_slots = (unsigned)n_slots;
+        lk->n_light = (unsigned)light.size();
+        lk->n_light2 = (unsigned)n_light2;
+        lk->n_multi = (unsigned)n_multi;
         lk->lw = lw;
         lk->tiles = (unsigned)tiles;
+        lk->row = n_cols % piece ? LK_TAIL : n_cols * e % 128 ? LK_WHOLE : LK_LINES;
+        lk->by_position = by_position;
         *out = lk;
         return TRAMP_OK;
     } catch (const std::exception&) {
@@ -658,26 +838,41 @@ extern "C" int tramp_lookup_destroy(tramp_ctx* ctx, tramp_lookup* lk) {
     TRAMP_REQUIRE(ctx, lk && lk->device == ctx->device);     \
     TRAMP_REQUIRE(ctx, batch <= 65535)
 
-// the rows fill whole pieces: no tails to look after
-static bool lk_whole(const tramp_lookup* lk) { return lk->D % (16 / dtype_size(lk->dtype)) == 0; }
+// CALL(ROW) for the handle's kind of rows
+#define LK_BY_ROW(lk, CALL)               \
+    switch ((lk)->row) {                  \
+        case LK_TAIL: CALL(LK_TAIL);      \
+        case LK_WHOLE: CALL(LK_WHOLE);    \
+        default: CALL(LK_LINES);          \
+    }
+
+// Instances by XCD (lk_place): worth it while the last round of eight leaves few XCDs idle.
+static int lk_spread(size_t batch, size_t blocks) {
+    return batch > 1 && (batch + 7) / 8 * 8 * 7 <= batch * 8 && (batch + 7) / 8 * 8 * blocks < 0x7fffffffu;
+}
+static dim3 lk_grid(size_t batch, size_t blocks, int spread) {
+    return spread ? dim3((unsigned)((batch + 7) / 8 * 8 * blocks)) : dim3((unsigned)blocks, (unsigned)batch);
+}
 
 template <typename T>
 static int lookup_apply(tramp_ctx* ctx, const tramp_lookup* lk, size_t batch, const T* z, T* x) {
     constexpr size_t N = LkVec<T>::N;
     if (lk->D == 1) {
         const size_t nb = (lk->T + kBlock * N - 1) / (kBlock * N);
-        hipLaunchKernelGGL((lookup_apply1_kernel<T>), dim3((unsigned)nb, (unsigned)batch), dim3(kBlock), 0, ctx->stream, lk->V, lk->T,
-                           lk->s, lk->tok, z, x);
+        const int spread = lk_spread(batch, nb);
+        hipLaunchKernelGGL((lookup_apply1_kernel<T>), lk_grid(batch, nb, spread), dim3(kBlock), 0, ctx->stream, lk->V, lk->T, lk->s,
+                           (unsigned)nb, (unsigned)batch, spread, lk->tok, z, x);
     } else {
-        const size_t per = (size_t)4 * (kBlock >> lk->lw), nb = (lk->T + per - 1) / per * lk->tiles;
-        TRAMP_REQUIRE(ctx, nb < 0x7fffffffu);
-        dim3 grid((unsigned)nb, (unsigned)batch);
-        if (lk_whole(lk))
-            hipLaunchKernelGGL((lookup_apply_kernel<T, false>), grid, dim3(kBlock), 0, ctx->stream, lk->V, lk->D, lk->T, lk->s, lk->lw,
-                               lk->tiles, lk->tok, z, x);
-        else
-            hipLaunchKernelGGL((lookup_apply_kernel<T, true>), grid, dim3(kBlock), 0, ctx->stream, lk->V, lk->D, lk->T, lk->s, lk->lw,
-                               lk->tiles, lk->tok, z, x);
+        const size_t per = (size_t)4 * (kBlock >> lk->lw), nb = (lk->T + per - 1) / per;
+        TRAMP_REQUIRE(ctx, nb * lk->tiles < 0x7fffffffu);
+        const int spread = lk_spread(batch, nb * lk->tiles);
+        const dim3 grid = lk_grid(batch, nb * lk->tiles, spread);
+#define LK_CALL(ROW)                                                                                                                   \
+    hipLaunchKernelGGL((lookup_apply_kernel<T, ROW>), grid, dim3(kBlock), 0, ctx->stream, lk->V, lk->D, lk->T, lk->s, lk->lw, (unsigned)nb, \
+                       lk->tiles, (unsigned)batch, spread, lk->tok, z, x);                                                             \
+    break
+        LK_BY_ROW(lk, LK_CALL)
+#undef LK_CALL
     }
     TRAMP_LAUNCH_CHECK(ctx);
     return TRAMP_OK;
@@ -691,72 +886,112 @@ extern "C" int tramp_lookup_apply(tramp_ctx* ctx, tramp_lookup* lk, size_t batch
                                   : lookup_apply<float>(ctx, lk, batch, (const float*)z_d, (float*)x_d);
 }
 
-// sums over the runs and what MODE makes of them; ctx->ws holds [scalars | partial sums | r of the heavy runs]
-template <typename T, bool TAIL, int MODE>
-static int launch_rows(tramp_ctx* ctx, const tramp_lookup* lk, size_t batch, size_t ws_at, const LkScal* scal, const T* bz, const T* x,
+static LkScalArgs lk_scal_args(const tramp_lookup* lk, int dir, const double* az, const double* ax, double damping, const double* a_old) {
+    LkScalArgs q{};
+    q.cnt = lk->cnt;
+    q.az = az;
+    q.ax = ax;
+    q.a_old = a_old;
+    q.V = (double)lk->V;
+    q.T = (double)lk->T;
+    q.padded = (double)(lk->T - lk->seen);
+    q.s = lk->s;
+    q.damping = damping;
+    q.K = lk->K;
+    q.dir = dir;
+    return q;
+}
+
+// ctx->ws of a call: [scalars | partial sums | scale r of the heavy runs, or of all runs of two and more positions]
+struct LkWs {
+    LkScal* scal;
+    double* partials;
+    double* sr;
+};
+static int lk_workspace(tramp_ctx* ctx, const tramp_lookup* lk, size_t batch, bool forward, LkWs* w) {
+    const size_t n_scal = (batch * sizeof(LkScal) + 255) & ~(size_t)255, n_part = batch * lk->n_chunks * lk->D * sizeof(double);
+    const size_t n_sr = !forward ? 0 : batch * (lk->by_position ? lk->n_multi : lk->n_joins) * lk->D * sizeof(double);
+    int rc = tramp_ws_reserve(ctx, n_scal + n_part + n_sr);
+    if (rc) return rc;
+    char* m = reinterpret_cast<char*>(ctx->ws);
+    *w = LkWs{reinterpret_cast<LkScal*>(m), reinterpret_cast<double*>(m + n_scal), reinterpret_cast<double*>(m + n_scal + n_part)};
+    return TRAMP_OK;
+}
+
+template <typename T, int ROW, int MODE>
+static int launch_rows(tramp_ctx* ctx, const tramp_lookup* lk, size_t batch, const LkWs& w, const LkScalArgs* q, const T* bz, const T* x,
                        double damping, const T* b_old, T* out, T* r_out) {
-    double* partials = reinterpret_cast<double*>(reinterpret_cast<char*>(ctx->ws) + ws_at);
-    double* r_ws = partials + batch * lk->n_slots * lk->D;
     LkArgs a{};
     a.off = lk->off;
     a.perm = lk->perm;
-    a.items = lk->items;
+    a.chunks = lk->chunks;
+    a.joins = lk->joins;
+    a.runs = lk->runs;
     a.waves = lk->waves;
+    a.light = MODE == LK_FWD || MODE == LK_MEAN ? lk->light : nullptr;
+    a.idx = lk->idx;
     a.V = lk->V;
     a.D = lk->D;
     a.T = lk->T;
-    a.n_items = lk->n_items;
+    a.n_chunks = lk->n_chunks;
+    a.n_joins = lk->n_joins;
+    a.n_runs = lk->n_runs;
     a.n_waves = lk->n_waves;
     a.wave_blocks = (lk->n_waves + kBlock / kWave - 1) / (kBlock / kWave);
+    a.n_light = MODE == LK_FWD ? lk->n_light : MODE == LK_MEAN ? lk->n_light2 : (unsigned)lk->V;
+    a.n_multi = lk->n_multi;
     a.tiles = lk->tiles;
-    a.n_slots = lk->n_slots;
+    a.batch = (unsigned)batch;
     a.lw = lk->lw;
     a.s = lk->s;
     const size_t G = kBlock >> lk->lw;
-    const size_t blocks = lk->n_items + a.wave_blocks + (lk->V + G - 1) / G;
-    TRAMP_REQUIRE(ctx, blocks * lk->tiles < 0x7fffffffu && (size_t)lk->n_spreads * lk->tiles < 0x7fffffffu);
+    const size_t blocks = (size_t)a.n_joins + a.n_runs + a.wave_blocks + ((size_t)a.n_light + G - 1) / G;
+    TRAMP_REQUIRE(ctx, blocks * lk->tiles < 0x7fffffffu && (size_t)lk->n_spreads * lk->tiles < 0x7fffffffu &&
+                           (size_t)lk->n_chunks * lk->tiles < 0x7ffffffeu);
+    if (lk->n_chunks || q)
+        hipLaunchKernelGGL((lookup_chunks_kernel<T, ROW, MODE != LK_FWD && MODE != LK_MEAN>), dim3(lk->n_chunks * lk->tiles + (q ? 1 : 0), (unsigned)batch),
+                           dim3(kBlock), 0, ctx->stream, a, q ? *q : LkScalArgs{}, x, w.partials);
     a.blocks = (unsigned)blocks;
-    hipLaunchKernelGGL((lookup_rows_kernel<T, TAIL, MODE>), dim3((unsigned)(blocks * lk->tiles), (unsigned)batch), dim3(kBlock), 0,
-                       ctx->stream, a, scal, bz, x, damping, b_old, out, r_out, partials);
-    if (lk->n_joins)
-        hipLaunchKernelGGL((lookup_join_kernel<T, TAIL, MODE>), dim3(lk->n_joins * lk->tiles, (unsigned)batch), dim3(kBlock), 0,
-                           ctx->stream, a, lk->joins, lk->n_joins, scal, bz, partials, damping, b_old, out, r_out, r_ws);
+    a.spread = lk_spread(batch, blocks * lk->tiles);
+    if (blocks)
+        hipLaunchKernelGGL((lookup_rows_kernel<T, ROW, MODE>), lk_grid(batch, blocks * lk->tiles, a.spread), dim3(kBlock), 0, ctx->stream, a,
+                           w.scal, bz, x, damping, b_old, out, r_out, w.partials, w.sr);
     if (MODE == LK_FWD && lk->n_spreads)
-        hipLaunchKernelGGL((lookup_spread_kernel<T, TAIL>), dim3(lk->n_spreads * lk->tiles, (unsigned)batch), dim3(kBlock), 0,
-                           ctx->stream, a, lk->spreads, lk->n_joins, scal, r_ws, x, damping, b_old, out, r_out);
+        hipLaunchKernelGGL((lookup_spread_kernel<T, ROW>), dim3(lk->n_spreads * lk->tiles, (unsigned)batch), dim3(kBlock), 0, ctx->stream, a,
+                           lk->spreads, w.scal, w.sr, x, damping, b_old, out, r_out);
+    if (MODE == LK_MEAN) {
+        const size_t per = lk->D == 1 ? (size_t)kBlock * LkVec<T>::N : 4 * G, nb = (lk->T + per - 1) / per;
+        a.blocks = (unsigned)nb;
+        a.spread = lk_spread(batch, nb * lk->tiles);
+        if (lk->D == 1)
+            hipLaunchKernelGGL((lookup_positions1_kernel<T>), lk_grid(batch, nb, a.spread), dim3(kBlock), 0, ctx->stream, a, lk->code, w.scal,
+                               bz, w.sr, x, damping, b_old, out, r_out);
+        else
+            hipLaunchKernelGGL((lookup_positions_kernel<T, ROW>), lk_grid(batch, nb * lk->tiles, a.spread), dim3(kBlock), 0, ctx->stream, a,
+                               lk->code, w.scal, bz, w.sr, x, damping, b_old, out, r_out);
+    }
     TRAMP_LAUNCH_CHECK(ctx);
     return TRAMP_OK;
 }
 
-static size_t scal_bytes(size_t batch) { return (batch * sizeof(LkScal) + 255) & ~(size_t)255; }
-
-static int lookup_ws(tramp_ctx* ctx, const tramp_lookup* lk, size_t batch) {
-    return tramp_ws_reserve(ctx, scal_bytes(batch) + batch * ((size_t)lk->n_slots + lk->n_joins) * lk->D * sizeof(double));
-}
-
 template <typename T, int MODE>
-static int run_rows(tramp_ctx* ctx, const tramp_lookup* lk, size_t batch, const LkScal* scal, const T* bz, const T* x, double damping,
-                    const T* b_old, T* out, T* r_out) {
-    return lk_whole(lk) ? launch_rows<T, false, MODE>(ctx, lk, batch, scal_bytes(batch), scal, bz, x, damping, b_old, out, r_out)
-                        : launch_rows<T, true, MODE>(ctx, lk, batch, scal_bytes(batch), scal, bz, x, damping, b_old, out, r_out);
+static int run_rows(tramp_ctx* ctx, const tramp_lookup* lk, size_t batch, const LkWs& w, const LkScalArgs* q, const T* bz, const T* x,
+                    double damping, const T* b_old, T* out, T* r_out) {
+#define LK_CALL(ROW) return launch_rows<T, ROW, MODE>(ctx, lk, batch, w, q, bz, x, damping, b_old, out, r_out)
+    LK_BY_ROW(lk, LK_CALL)
+#undef LK_CALL
 }
 
 extern "C" int tramp_lookup_gradient(tramp_ctx* ctx, tramp_lookup* lk, size_t batch, const void* x_d, void* g_d) {
     LK_REQUIRE_CALL(ctx, lk, batch);
     TRAMP_REQUIRE(ctx, x_d && g_d && x_d != g_d);
     if (!batch) return TRAMP_OK;
-    int rc = lookup_ws(ctx, lk, batch);
+    LkWs w;
+    int rc = lk_workspace(ctx, lk, batch, false, &w);
     if (rc) return rc;
     if (lk->dtype == TRAMP_F64)
-        return run_rows<double, LK_GRAD>(ctx, lk, batch, nullptr, nullptr, (const double*)x_d, 0.0, nullptr, (double*)g_d, nullptr);
-    return run_rows<float, LK_GRAD>(ctx, lk, batch, nullptr, nullptr, (const float*)x_d, 0.0, nullptr, (float*)g_d, nullptr);
-}
-
-static void launch_scalars(tramp_ctx* ctx, const tramp_lookup* lk, int dir, size_t batch, const double* az_d, const double* ax_d,
-                           double damping, const double* a_old_d, LkScal* scal, double* v_d, double* a_new_d, double* n_eff_d) {
-    hipLaunchKernelGGL(lookup_scalars_kernel, dim3((unsigned)batch), dim3(kBlock), 0, ctx->stream, lk->K, lk->cnt, (double)lk->V,
-                       (double)lk->T, (double)(lk->T - lk->seen), lk->s, dir, az_d, ax_d, damping, a_old_d, scal, v_d, a_new_d,
-                       n_eff_d);
+        return run_rows<double, LK_GRAD>(ctx, lk, batch, w, nullptr, nullptr, (const double*)x_d, 0.0, nullptr, (double*)g_d, nullptr);
+    return run_rows<float, LK_GRAD>(ctx, lk, batch, w, nullptr, nullptr, (const float*)x_d, 0.0, nullptr, (float*)g_d, nullptr);
 }
 
 extern "C" int tramp_lookup_variance(tramp_ctx* ctx, tramp_lookup* lk, int dir, size_t batch, const double* az_d,
@@ -764,7 +999,11 @@ extern "C" int tramp_lookup_variance(tramp_ctx* ctx, tramp_lookup* lk, int dir, 
     LK_REQUIRE_CALL(ctx, lk, batch);
     TRAMP_REQUIRE(ctx, (dir == TRAMP_FWD || dir == TRAMP_BWD) && az_d && ax_d);
     if (!batch) return TRAMP_OK;
-    launch_scalars(ctx, lk, dir, batch, az_d, ax_d, 0.0, nullptr, nullptr, v_d, a_new_d, n_eff_d);
+    LkScalArgs q = lk_scal_args(lk, dir, az_d, ax_d, 0.0, nullptr);
+    q.v_out = v_d;
+    q.a_new_out = a_new_d;
+    q.n_eff_out = n_eff_d;
+    hipLaunchKernelGGL(lookup_scalars_kernel, dim3((unsigned)batch), dim3(kBlock), 0, ctx->stream, q);
     TRAMP_LAUNCH_CHECK(ctx);
     return TRAMP_OK;
 }
@@ -773,12 +1012,16 @@ template <typename T>
 static int lookup_message(tramp_ctx* ctx, tramp_lookup* lk, int dir, size_t batch, const double* az_d, const T* bz,
                           const double* ax_d, const T* bx, double damping, const double* a_old_d, const T* b_old, double* a_new_d,
                           T* b_new, T* r_d, double* v_d) {
-    int rc = lookup_ws(ctx, lk, batch);
+    LkWs w;
+    int rc = lk_workspace(ctx, lk, batch, dir == TRAMP_FWD, &w);
     if (rc) return rc;
-    LkScal* scal = reinterpret_cast<LkScal*>(ctx->ws);
-    launch_scalars(ctx, lk, dir, batch, az_d, ax_d, damping, a_old_d, scal, v_d, a_new_d, nullptr);
-    return dir == TRAMP_BWD ? run_rows<T, LK_BWD>(ctx, lk, batch, scal, bz, bx, damping, b_old, b_new, r_d)
-                            : run_rows<T, LK_FWD>(ctx, lk, batch, scal, bz, bx, damping, b_old, b_new, r_d);
+    LkScalArgs q = lk_scal_args(lk, dir, az_d, ax_d, damping, a_old_d);
+    q.scal = w.scal;
+    q.v_out = v_d;
+    q.a_new_out = a_new_d;
+    if (dir == TRAMP_BWD) return run_rows<T, LK_BWD>(ctx, lk, batch, w, &q, bz, bx, damping, b_old, b_new, r_d);
+    if (lk->by_position) return run_rows<T, LK_MEAN>(ctx, lk, batch, w, &q, bz, bx, damping, b_old, b_new, r_d);
+    return run_rows<T, LK_FWD>(ctx, lk, batch, w, &q, bz, bx, damping, b_old, b_new, r_d);
 }
 
 extern "C" int tramp_lookup_message(tramp_ctx* ctx, tramp_lookup* lk, int dir, size_t batch, const double* az_d, const void* bz_d,
