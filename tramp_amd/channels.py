@@ -1621,8 +1621,12 @@ class LookupChannel(Channel):
         ctx = self.ctx
         z, x, a_z, a_x = self._args(az, bz, ax, bx)
         tgt, a_t = (x, a_x) if direction == _lib.FWD else (z, a_z)
-        a_new = out_a if out_a is not None else ctx.empty((z.batch,), np.float64)
-        b_new = self._out(out_b, z.batch, tgt.n, self.dtype)
+        a_new, b_new = self._out(out_a, z.batch, 1, np.float64), self._out(out_b, z.batch, tgt.n, self.dtype)
+        if damping:
+            if old_a is None or old_b is None:
+                raise ValueError("damping needs old_a and old_b")
+            self._out(old_a, z.batch, 1, np.float64)
+            self._out(old_b, z.batch, tgt.n, self.dtype)
         r = ctx.empty((z.batch, tgt.n), self.dtype) if want_posterior else None
         v = ctx.empty((z.batch,), np.float64) if want_posterior else None
         ctx._call("tramp_lookup_message", self._handle, direction, z.batch, a_z.dev.ptr, z.dev.ptr, a_x.dev.ptr, x.dev.ptr,

@@ -2,7 +2,7 @@
 // bounded step new <- old + min(1, max / |new - old|) (new - old) of a whole set of EP messages.
 //
 // The arrays of a list have lengths of their own, [batch, n_i] each; an instance b owns row b of every array.  The list is laid
-// out once as chunks of 32 KiB that never straddle two arrays; workgroup p of instance b walks the chunks p, p + P, ... and
+// out once as chunks of 16 KiB that never straddle two arrays; workgroup p of instance b walks the chunks p, p + P, ... and
 // leaves one partial sum of squares, the second launch adds the P partials of its instance in a fixed order (every workgroup
 // for itself: P <= 2048 doubles out of the L2) and applies the factor, from the last chunk to the first: what the first pass
 // read last is still in the 256 MB of cache before memory.  Sums are held in double: no overflow below 1e154, no loss in long
@@ -14,9 +14,21 @@
 #include <vector>
 
 namespace {
-constexpr size_t kChunkBytes = 32768;                // 8 pieces of 16 bytes per thread
+constexpr size_t kChunkBytes = 16384;                // 4 pieces of 16 bytes per thread
 constexpr int kPieces = kChunkBytes / 16 / kBlock;
-constexpr int kMaxPartials = 2048;
+// Up to this many chunks one workgroup does both passes of an instance, in one launch: 4 arrays of 1000 f64 together 5.4 against
+// 7.6 us, of 3000 6.3 against 7.9 us; 12000 (six chunks) would be 11.8 against 7.6 us.
+constexpr size_t kSmall = 4;
+// workgroups of a pass: 8 per CU; 1280 and 4096 time the same within 4 % (24 arrays of 10^9 bytes), 1280 loses 20 % on 64
+// instances
+constexpr size_t kBlocks = 2048;
+// Lists larger than this are gone from the cache before anyone reads the result: the second pass reads and writes past it.
+// 10^9 bytes 559 -> 494 us, 64 instances x 300000 f64 with their previous values 140 -> 130 us, 16 x 3000000 f32 112 -> 101 us;
+// 20 MB 14.4 -> 15.3 us.
+constexpr size_t kOnce = (size_t)128 << 20;
+// Slices of instances (group_run): 64 instances x 300000 f64 and their previous values, 307 MB, in slices of 80 MB 140 us, of
+// 48 MB 151 us, of 128 MB 143 us, whole 152 us.
+constexpr size_t kSlice = (size_t)80 << 20;
 }  // namespace
 
 // one chunk: everything a workgroup needs in one scalar load, the next one's is on its way while this one is worked on
@@ -34,8 +46,11 @@ struct tramp_group {
     size_t nchunk;
     void* mem;
     const GroupChunk* chunks;    // [nchunk]; lists of the same lengths have the same chunks
-    void** ptr_h;                // host copies (checks between lists)
+    // host copies for the checks between lists: the arrays in order, and where they lie, sorted
+    void** ptr_h;
     size_t* len_h;
+    struct Span { uintptr_t lo, hi; }* span;
+    int n_span;
 };
 
 // 16-byte pieces at any element boundary
@@ -49,43 +64,52 @@ template <> struct GVec<double> {
     static constexpr int N = 2;
 };
 
-// partial sums of squares of x (STEP = false) or of x - prev
+// ONCE: past the caches, for what will not be touched again before it is gone from them
+template <typename T, bool ONCE> __device__ __forceinline__ typename GVec<T>::U g_load(const T* p, unsigned j) {
+    using U = typename GVec<T>::U;
+    return ONCE ? __builtin_nontemporal_load(reinterpret_cast<const U*>(p) + j) : reinterpret_cast<const U*>(p)[j];
+}
+template <typename T, bool ONCE> __device__ __forceinline__ void g_store(T* p, unsigned j, typename GVec<T>::U v) {
+    using U = typename GVec<T>::U;
+    if (ONCE)
+        __builtin_nontemporal_store(v, reinterpret_cast<U*>(p) + j);
+    else
+        reinterpret_cast<U*>(p)[j] = v;
+}
+
+// sum of squares of a chunk of x (STEP = false) or of x - prev, this thread's share
 template <typename T, bool STEP>
-__global__ __launch_bounds__(kBlock) void group_squares_kernel(unsigned nchunk, const GroupChunk* __restrict__ xs, const GroupChunk* __restrict__ ps,
-                                                               double* __restrict__ partials) {
+__device__ __forceinline__ double chunk_squares(const GroupChunk* __restrict__ xs, const GroupChunk* __restrict__ ps, size_t b) {
     using U = typename GVec<T>::U;
     constexpr int N = GVec<T>::N;
-    constexpr size_t CH = kChunkBytes / sizeof(T);
-    __shared__ double smem[kBlock / kWave];
-    const size_t b = blockIdx.y;
+    const T* x = reinterpret_cast<const T*>(xs->addr + b * xs->stride);
+    const T* p = STEP ? reinterpret_cast<const T*>(ps->addr + b * ps->stride) : nullptr;
+    const unsigned len = xs->len, full = len / N;
+    U v[kPieces], w[kPieces];
     double acc = 0.0;
-    for (unsigned c = blockIdx.x; c < nchunk; c += gridDim.x) {
-        const T* x = reinterpret_cast<const T*>(xs[c].addr + b * xs[c].stride);
-        const T* p = STEP ? reinterpret_cast<const T*>(ps[c].addr + b * ps[c].stride) : nullptr;
-        const size_t len = xs[c].len;
-        if (len == CH) {
-            U v[kPieces], w[kPieces];
 #pragma unroll
-            for (int i = 0; i < kPieces; ++i) {
-                v[i] = reinterpret_cast<const U*>(x)[i * kBlock + threadIdx.x];
-                if (STEP) w[i] = reinterpret_cast<const U*>(p)[i * kBlock + threadIdx.x];
-            }
+    for (int i = 0; i < kPieces; ++i) {
+        const unsigned j = i * kBlock + threadIdx.x;
+        if (j < full) {
+            v[i] = reinterpret_cast<const U*>(x)[j];
+            if (STEP) w[i] = reinterpret_cast<const U*>(p)[j];
+        }
+    }
+    const unsigned r = full * N + threadIdx.x;                     // fewer than N elements behind the whole pieces
+    if (r < len) {
+        const double d = STEP ? (double)x[r] - (double)p[r] : (double)x[r];
+        acc = fma(d, d, acc);
+    }
 #pragma unroll
-            for (int i = 0; i < kPieces; ++i)
+    for (int i = 0; i < kPieces; ++i)
+        if (i * kBlock + threadIdx.x < full) {
 #pragma unroll
-                for (int e = 0; e < N; ++e) {
-                    const double d = STEP ? (double)v[i][e] - (double)w[i][e] : (double)v[i][e];
-                    acc = fma(d, d, acc);
-                }
-        } else {
-            for (size_t j = threadIdx.x; j < len; j += kBlock) {
-                const double d = STEP ? (double)x[j] - (double)p[j] : (double)x[j];
+            for (int e = 0; e < N; ++e) {
+                const double d = STEP ? (double)v[i][e] - (double)w[i][e] : (double)v[i][e];
                 acc = fma(d, d, acc);
             }
         }
-    }
-    acc = block_sum(acc, smem);
-    if (threadIdx.x == 0) partials[b * gridDim.x + blockIdx.x] = acc;
+    return acc;
 }
 
 __device__ __forceinline__ double fold_norm(const double* __restrict__ partials, int P, size_t b, double* smem) {
@@ -110,57 +134,99 @@ template <typename T, bool STEP> __device__ __forceinline__ T bounded(T x, T p, 
     return STEP ? T((double)p + c * ((double)x - (double)p)) : T(c * (double)x);
 }
 
-// out = c x, or out = prev + c (x - prev) with the precisions a moved by the same factor; refresh: the result over prev too
-template <typename T, bool STEP>
-__global__ __launch_bounds__(kBlock) void group_apply_kernel(unsigned nchunk, const GroupChunk* __restrict__ xs, const GroupChunk* __restrict__ ps,
-                                                             const GroupChunk* __restrict__ os, int refresh, double bound,
-                                                             const double* __restrict__ partials, int P, size_t n_a, size_t B, double* a,
-                                                             double* a_prev, double* __restrict__ norm_out) {
+// one chunk of out = c x, or of out = prev + c (x - prev); refresh: the result over prev too
+template <typename T, bool STEP, bool ONCE>
+__device__ __forceinline__ void chunk_apply(const GroupChunk* __restrict__ xs, const GroupChunk* __restrict__ ps,
+                                            const GroupChunk* __restrict__ os, size_t b, int refresh, double c) {
     using U = typename GVec<T>::U;
     constexpr int N = GVec<T>::N;
-    constexpr size_t CH = kChunkBytes / sizeof(T);
-    __shared__ double smem[kBlock / kWave];
-    const size_t b = blockIdx.y;
-    const double norm = fold_norm(partials, P, b, smem), c = clip_factor(norm, bound);
-    if (blockIdx.x == 0) {
-        if (threadIdx.x == 0 && norm_out) norm_out[b] = norm;
-        if (STEP)
-            for (size_t i = threadIdx.x; i < n_a; i += kBlock) {
-                const double o = a_prev[i * B + b];
-                const double r = c < 1.0 ? o + c * (a[i * B + b] - o) : a[i * B + b];
-                a[i * B + b] = r;
-                if (refresh) a_prev[i * B + b] = r;
-            }
-    }
-    for (unsigned k = blockIdx.x; k < nchunk; k += gridDim.x) {
-        const unsigned ch = nchunk - 1 - k;
-        const T* x = reinterpret_cast<const T*>(xs[ch].addr + b * xs[ch].stride);
-        T* p = STEP ? reinterpret_cast<T*>(ps[ch].addr + b * ps[ch].stride) : nullptr;
-        T* o = reinterpret_cast<T*>(os[ch].addr + b * os[ch].stride);
-        const size_t len = xs[ch].len;
-        if (c == 1.0 && o == x && !(STEP && refresh)) continue;
-        if (len == CH) {
-            U v[kPieces], w[kPieces];
+    const T* x = reinterpret_cast<const T*>(xs->addr + b * xs->stride);
+    T* p = STEP ? reinterpret_cast<T*>(ps->addr + b * ps->stride) : nullptr;
+    T* o = reinterpret_cast<T*>(os->addr + b * os->stride);
+    if (c == 1.0 && o == x && !(STEP && refresh)) return;
+    const unsigned len = xs->len, full = len / N;
+    U v[kPieces], w[kPieces];
 #pragma unroll
-            for (int i = 0; i < kPieces; ++i) {
-                v[i] = reinterpret_cast<const U*>(x)[i * kBlock + threadIdx.x];
-                if (STEP) w[i] = reinterpret_cast<const U*>(p)[i * kBlock + threadIdx.x];
-            }
-#pragma unroll
-            for (int i = 0; i < kPieces; ++i) {
-#pragma unroll
-                for (int e = 0; e < N; ++e) v[i][e] = bounded<T, STEP>(v[i][e], STEP ? w[i][e] : T(0), c);
-                reinterpret_cast<U*>(o)[i * kBlock + threadIdx.x] = v[i];
-                if (STEP && refresh) reinterpret_cast<U*>(p)[i * kBlock + threadIdx.x] = v[i];
-            }
-        } else {
-            for (size_t j = threadIdx.x; j < len; j += kBlock) {
-                const T r = bounded<T, STEP>(x[j], STEP ? p[j] : T(0), c);
-                o[j] = r;
-                if (STEP && refresh) p[j] = r;
-            }
+    for (int i = 0; i < kPieces; ++i) {
+        const unsigned j = i * kBlock + threadIdx.x;
+        if (j < full) {
+            v[i] = g_load<T, ONCE>(x, j);
+            if (STEP) w[i] = g_load<T, ONCE>(p, j);
         }
     }
+    const unsigned r = full * N + threadIdx.x;
+    if (r < len) {
+        const T t = bounded<T, STEP>(x[r], STEP ? p[r] : T(0), c);
+        o[r] = t;
+        if (STEP && refresh) p[r] = t;
+    }
+#pragma unroll
+    for (int i = 0; i < kPieces; ++i) {
+        const unsigned j = i * kBlock + threadIdx.x;
+        if (j < full) {
+#pragma unroll
+            for (int e = 0; e < N; ++e) v[i][e] = bounded<T, STEP>(v[i][e], STEP ? w[i][e] : T(0), c);
+            g_store<T, ONCE>(o, j, v[i]);
+            if (STEP && refresh) g_store<T, ONCE>(p, j, v[i]);
+        }
+    }
+}
+
+// what goes with the arrays: the norm, the precisions a moved by the same factor
+struct GroupSide {
+    double bound;
+    double* norm_out;
+    double* a;
+    double* a_prev;
+    size_t n_a, batch;
+    int refresh;
+};
+template <bool STEP> __device__ __forceinline__ void group_side(const GroupSide& q, size_t b, double norm, double c) {
+    if (threadIdx.x == 0 && q.norm_out) q.norm_out[b] = norm;
+    if (!STEP) return;
+    for (size_t i = threadIdx.x; i < q.n_a; i += kBlock) {
+        const double o = q.a_prev[i * q.batch + b], x = q.a[i * q.batch + b];
+        const double r = c < 1.0 ? o + c * (x - o) : x;
+        q.a[i * q.batch + b] = r;
+        if (q.refresh) q.a_prev[i * q.batch + b] = r;
+    }
+}
+
+// The two passes.  Rows y of the grid: the instances [a0, a0 + n_apply), whose sums an earlier launch has left, are finished;
+// of the following ones the sums are taken.
+template <typename T, bool STEP, bool ONCE>
+__global__ __launch_bounds__(kBlock) void group_pass_kernel(unsigned nchunk, const GroupChunk* __restrict__ xs, const GroupChunk* __restrict__ ps,
+                                                            const GroupChunk* __restrict__ os, size_t a0, unsigned n_apply, GroupSide q,
+                                                            double* __restrict__ partials) {
+    __shared__ double smem[kBlock / kWave];
+    const size_t b = a0 + blockIdx.y;
+    if (blockIdx.y >= n_apply) {
+        double acc = 0.0;
+        for (unsigned c = blockIdx.x; c < nchunk; c += gridDim.x) acc += chunk_squares<T, STEP>(xs + c, ps + c, b);
+        acc = block_sum(acc, smem);
+        if (threadIdx.x == 0) partials[b * gridDim.x + blockIdx.x] = acc;
+        return;
+    }
+    const double norm = fold_norm(partials, gridDim.x, b, smem), c = clip_factor(norm, q.bound);
+    if (blockIdx.x == 0) group_side<STEP>(q, b, norm, c);
+    for (unsigned k = blockIdx.x; k < nchunk; k += gridDim.x) {
+        const unsigned ch = nchunk - 1 - k;
+        chunk_apply<T, STEP, ONCE>(xs + ch, ps + ch, os + ch, b, q.refresh, c);
+    }
+}
+
+// small instances: one workgroup each does both passes in one launch
+template <typename T, bool STEP>
+__global__ __launch_bounds__(kBlock) void group_small_kernel(unsigned nchunk, const GroupChunk* __restrict__ xs, const GroupChunk* __restrict__ ps,
+                                                             const GroupChunk* __restrict__ os, GroupSide q) {
+    __shared__ double smem[kBlock / kWave];
+    const size_t b = blockIdx.x;
+    double acc = 0.0;
+    for (unsigned c = 0; c < nchunk; ++c) acc += chunk_squares<T, STEP>(xs + c, ps + c, b);
+    const double norm = sqrt(block_sum(acc, smem)), c = clip_factor(norm, q.bound);
+    group_side<STEP>(q, b, norm, c);
+    if (!os) return;
+    for (unsigned k = 0; k < nchunk; ++k) chunk_apply<T, STEP, false>(xs + k, ps + k, os + k, b, q.refresh, c);
 }
 
 // ---------------------------------------------------------------- handle
@@ -175,18 +241,18 @@ extern "C" int tramp_group_create(tramp_ctx* ctx, int dtype, int k, void* const*
     const size_t e = dtype_size(dtype), per = kChunkBytes / e;
     try {
         size_t nchunk = 0;
-        std::vector<std::pair<uintptr_t, uintptr_t>> span;
+        std::vector<tramp_group::Span> span;
         for (int i = 0; i < k; ++i) {
             TRAMP_REQUIRE(ctx, arrays_d[i] || !n[i]);
             TRAMP_REQUIRE(ctx, n[i] <= ((size_t)1 << 40) / batch);
             nchunk += (n[i] + per - 1) / per;
             const uintptr_t a = (uintptr_t)arrays_d[i];
-            if (n[i]) span.emplace_back(a, a + n[i] * batch * e);
+            if (n[i]) span.push_back({a, a + n[i] * batch * e});
         }
         TRAMP_REQUIRE(ctx, nchunk < 0x7fffffffu);
-        std::sort(span.begin(), span.end());
+        std::sort(span.begin(), span.end(), [](const tramp_group::Span& a, const tramp_group::Span& b) { return a.lo < b.lo; });
         for (size_t i = 1; i < span.size(); ++i)
-            if (span[i].first < span[i - 1].second)
+            if (span[i].lo < span[i - 1].hi)
                 return tramp_fail(ctx, TRAMP_EINVAL, "tramp_group_create", "two arrays of the list overlap");
         std::vector<GroupChunk> chunks;
         chunks.reserve(nchunk);
@@ -200,11 +266,13 @@ extern "C" int tramp_group_create(tramp_ctx* ctx, int dtype, int k, void* const*
         *g = tramp_group{};
         g->ptr_h = static_cast<void**>(malloc((size_t)k * 8));
         g->len_h = static_cast<size_t*>(malloc((size_t)k * 8));
+        g->span = static_cast<tramp_group::Span*>(malloc((size_t)k * sizeof(tramp_group::Span)));
         (void)hipSetDevice(ctx->device);
-        if (!g->ptr_h || !g->len_h || hipMalloc(&g->mem, total) != hipSuccess) {
+        if (!g->ptr_h || !g->len_h || !g->span || hipMalloc(&g->mem, total) != hipSuccess) {
             (void)hipGetLastError();
             free(g->ptr_h);
             free(g->len_h);
+            free(g->span);
             delete g;
             return tramp_fail(ctx, TRAMP_ENOMEM, "tramp_group_create", "out of memory");
         }
@@ -214,11 +282,14 @@ extern "C" int tramp_group_create(tramp_ctx* ctx, int dtype, int k, void* const*
             (void)hipFree(g->mem);
             free(g->ptr_h);
             free(g->len_h);
+            free(g->span);
             delete g;
             return tramp_fail(ctx, TRAMP_EHIP, "tramp_group_create", hipGetErrorString(err));
         }
         memcpy(g->ptr_h, arrays_d, (size_t)k * 8);
         memcpy(g->len_h, n, (size_t)k * 8);
+        std::copy(span.begin(), span.end(), g->span);
+        g->n_span = (int)span.size();
         g->device = ctx->device;
         g->dtype = dtype;
         g->k = k;
@@ -238,6 +309,7 @@ extern "C" int tramp_group_destroy(tramp_ctx* ctx, tramp_group* g) {
     (void)hipFree(g->mem);
     free(g->ptr_h);
     free(g->len_h);
+    free(g->span);
     delete g;
     return TRAMP_OK;
 }
@@ -250,42 +322,56 @@ static int check_pair(tramp_ctx* ctx, const tramp_group* g, const tramp_group* o
     for (int i = 0; i < g->k; ++i)
         if (o->len_h[i] != g->len_h[i]) return tramp_fail(ctx, TRAMP_EINVAL, what, "arrays of different lengths");
     if (g == o) return same ? TRAMP_OK : tramp_fail(ctx, TRAMP_EINVAL, what, "the same list twice");
-    try {
-        std::vector<std::pair<uintptr_t, uintptr_t>> span;
-        for (int i = 0; i < g->k; ++i)
-            if (g->len_h[i]) span.emplace_back((uintptr_t)g->ptr_h[i], (uintptr_t)g->ptr_h[i] + g->len_h[i] * g->batch * e);
-        std::sort(span.begin(), span.end());
-        for (int i = 0; i < g->k; ++i) {
-            if (!g->len_h[i] || (same && o->ptr_h[i] == g->ptr_h[i])) continue;
-            const uintptr_t lo = (uintptr_t)o->ptr_h[i], hi = lo + g->len_h[i] * g->batch * e;
-            auto it = std::upper_bound(span.begin(), span.end(), std::make_pair(hi - 1, (uintptr_t)-1));
-            if (it != span.begin() && std::prev(it)->second > lo)
-                return tramp_fail(ctx, TRAMP_EINVAL, what, "the arrays of the two lists overlap");
-        }
-    } catch (const std::bad_alloc&) {
-        return tramp_fail(ctx, TRAMP_ENOMEM, what, "host memory");
+    for (int i = 0; i < g->k; ++i) {
+        if (!g->len_h[i] || (same && o->ptr_h[i] == g->ptr_h[i])) continue;
+        const uintptr_t lo = (uintptr_t)o->ptr_h[i], hi = lo + g->len_h[i] * g->batch * e;
+        // the last array of g that starts before hi ends last of those
+        const tramp_group::Span* it = std::lower_bound(g->span, g->span + g->n_span, hi, [](const tramp_group::Span& s, uintptr_t x) { return s.lo < x; });
+        if (it != g->span && (it - 1)->hi > lo) return tramp_fail(ctx, TRAMP_EINVAL, what, "the arrays of the two lists overlap");
     }
     return TRAMP_OK;
 }
 
-static int partials_of(const tramp_group* g) {
-    return (int)(g->nchunk < 1 ? 1 : g->nchunk > (size_t)kMaxPartials ? (size_t)kMaxPartials : g->nchunk);
+// workgroups per instance: about kBlocks in all, each with the same number of chunks
+static int partials_of(const tramp_group* g, size_t batch) {
+    if (g->nchunk < 1) return 1;
+    const size_t want = std::max((size_t)1, kBlocks / batch), rounds = (g->nchunk + want - 1) / want;
+    return (int)((g->nchunk + rounds - 1) / rounds);
 }
 
 template <typename T, bool STEP>
-static int group_run(tramp_ctx* ctx, const tramp_group* g, const tramp_group* prev, const tramp_group* out, int refresh, double bound,
-                     size_t n_a, double* a, double* a_prev, double* norm_d) {
-    const int P = partials_of(g);
+static int group_run(tramp_ctx* ctx, const tramp_group* g, const tramp_group* prev, const tramp_group* out, const GroupSide& q) {
+    const GroupChunk* ps = STEP ? prev->chunks : nullptr;
+    if (g->nchunk <= kSmall) {
+        hipLaunchKernelGGL((group_small_kernel<T, STEP>), dim3((unsigned)g->batch), dim3(kBlock), 0, ctx->stream, (unsigned)g->nchunk, g->chunks,
+                           ps, out ? out->chunks : nullptr, q);
+        TRAMP_LAUNCH_CHECK(ctx);
+        return TRAMP_OK;
+    }
+    // Instances in slices whose arrays stay in the 256 MB of cache from one pass to the other: every launch finishes one slice and
+    // takes the sums of the next.
+    const size_t bytes = g->nchunk * kChunkBytes * (STEP ? 2 : 1), most = kSlice;
+    const size_t slice = !out || bytes * g->batch <= 2 * most || bytes > most ? g->batch : most / bytes;
+    const int P = partials_of(g, slice);
     int rc = tramp_ws_reserve(ctx, g->batch * (size_t)P * sizeof(double));
     if (rc) return rc;
-    dim3 grid((unsigned)P, (unsigned)g->batch);
-    hipLaunchKernelGGL((group_squares_kernel<T, STEP>), grid, dim3(kBlock), 0, ctx->stream, (unsigned)g->nchunk, g->chunks,
-                       STEP ? prev->chunks : nullptr, ctx->ws);
+    size_t done = 0, summed = 0;
+    while (done < g->batch) {
+        const size_t n_apply = out ? summed - done : 0, n_sum = std::min(slice, g->batch - summed);
+        const dim3 grid((unsigned)P, (unsigned)(n_apply + n_sum));
+        const GroupChunk* os = out ? out->chunks : nullptr;
+        if (bytes * g->batch > kOnce)
+            hipLaunchKernelGGL((group_pass_kernel<T, STEP, true>), grid, dim3(kBlock), 0, ctx->stream, (unsigned)g->nchunk, g->chunks, ps, os,
+                               done, (unsigned)n_apply, q, ctx->ws);
+        else
+            hipLaunchKernelGGL((group_pass_kernel<T, STEP, false>), grid, dim3(kBlock), 0, ctx->stream, (unsigned)g->nchunk, g->chunks, ps, os,
+                               done, (unsigned)n_apply, q, ctx->ws);
+        done = summed;
+        summed += n_sum;
+        if (!out) break;
+    }
     if (!out)
-        hipLaunchKernelGGL(group_norm_kernel, dim3((unsigned)g->batch), dim3(kBlock), 0, ctx->stream, ctx->ws, P, norm_d);
-    else
-        hipLaunchKernelGGL((group_apply_kernel<T, STEP>), grid, dim3(kBlock), 0, ctx->stream, (unsigned)g->nchunk, g->chunks,
-                           STEP ? prev->chunks : nullptr, out->chunks, refresh, bound, ctx->ws, P, n_a, g->batch, a, a_prev, norm_d);
+        hipLaunchKernelGGL(group_norm_kernel, dim3((unsigned)g->batch), dim3(kBlock), 0, ctx->stream, ctx->ws, P, q.norm_out);
     TRAMP_LAUNCH_CHECK(ctx);
     return TRAMP_OK;
 }
@@ -293,8 +379,9 @@ static int group_run(tramp_ctx* ctx, const tramp_group* g, const tramp_group* pr
 extern "C" int tramp_group_norm(tramp_ctx* ctx, const tramp_group* g, double* norm_d) {
     if (!ctx) return TRAMP_EINVAL;
     TRAMP_REQUIRE(ctx, g && norm_d && g->device == ctx->device);
-    return g->dtype == TRAMP_F64 ? group_run<double, false>(ctx, g, nullptr, nullptr, 0, 0.0, 0, nullptr, nullptr, norm_d)
-                                 : group_run<float, false>(ctx, g, nullptr, nullptr, 0, 0.0, 0, nullptr, nullptr, norm_d);
+    const GroupSide q{0.0, norm_d, nullptr, nullptr, 0, g->batch, 0};
+    return g->dtype == TRAMP_F64 ? group_run<double, false>(ctx, g, nullptr, nullptr, q)
+                                 : group_run<float, false>(ctx, g, nullptr, nullptr, q);
 }
 
 extern "C" int tramp_group_clip(tramp_ctx* ctx, const tramp_group* g, double max_norm, const tramp_group* out, double* norm_d) {
@@ -303,8 +390,9 @@ extern "C" int tramp_group_clip(tramp_ctx* ctx, const tramp_group* g, double max
     TRAMP_REQUIRE(ctx, max_norm > 0.0);
     int rc = check_pair(ctx, g, out, true, "tramp_group_clip");
     if (rc) return rc;
-    return g->dtype == TRAMP_F64 ? group_run<double, false>(ctx, g, nullptr, out, 0, max_norm, 0, nullptr, nullptr, norm_d)
-                                 : group_run<float, false>(ctx, g, nullptr, out, 0, max_norm, 0, nullptr, nullptr, norm_d);
+    const GroupSide q{max_norm, norm_d, nullptr, nullptr, 0, g->batch, 0};
+    return g->dtype == TRAMP_F64 ? group_run<double, false>(ctx, g, nullptr, out, q)
+                                 : group_run<float, false>(ctx, g, nullptr, out, q);
 }
 
 extern "C" int tramp_group_limit_step(tramp_ctx* ctx, const tramp_group* g, const tramp_group* prev, double max_step,
@@ -318,6 +406,7 @@ extern "C" int tramp_group_limit_step(tramp_ctx* ctx, const tramp_group* g, cons
     if (!rc) rc = check_pair(ctx, g, out, true, "tramp_group_limit_step");
     if (!rc) rc = check_pair(ctx, prev, out, false, "tramp_group_limit_step");
     if (rc) return rc;
-    return g->dtype == TRAMP_F64 ? group_run<double, true>(ctx, g, prev, out, refresh, max_step, n_a, a_d, a_prev_d, norm_d)
-                                 : group_run<float, true>(ctx, g, prev, out, refresh, max_step, n_a, a_d, a_prev_d, norm_d);
+    const GroupSide q{max_step, norm_d, a_d, a_prev_d, n_a, g->batch, refresh};
+    return g->dtype == TRAMP_F64 ? group_run<double, true>(ctx, g, prev, out, q)
+                                 : group_run<float, true>(ctx, g, prev, out, q);
 }

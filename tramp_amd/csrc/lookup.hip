@@ -52,7 +52,7 @@ struct tramp_lookup {
     int lw;                      // log2 of the lanes per row
     unsigned tiles;              // column tiles per row
     int row;                     // LK_TAIL / LK_WHOLE / LK_LINES
-    bool by_position;            // the message to x in the order of the positions
+    bool short_rows;             // under half a line: the message to x may go in the order of the positions
 };
 
 // what the kernels need of one instance, written by lk_scalars
@@ -76,7 +76,8 @@ struct LkScalArgs {
     int K, dir;
 };
 
-__device__ void lk_scalars(const LkScalArgs& q, size_t b) {
+// every workgroup that calls it ends with the same bits; `write`: this one stores them
+__device__ __forceinline__ LkScal lk_scalars(const LkScalArgs& q, size_t b, bool write) {
     __shared__ double smem[kBlock / kWave];
     const int K = q.K, dir = q.dir;
     const double* cnt = q.cnt;
@@ -100,7 +101,6 @@ __device__ void lk_scalars(const LkScalArgs& q, size_t b) {
     sv = block_sum(sv, smem);
     sn = block_sum(sn, smem);
     se = block_sum(se, smem);
-    if (threadIdx.x != 0) return;
     double v, an;
     if (dir == TRAMP_BWD) {
         v = sv / q.V;
@@ -112,13 +112,17 @@ __device__ void lk_scalars(const LkScalArgs& q, size_t b) {
     if (v > 1.7976931348623157e308) an = 0.0;                    // both precisions zero: 1 / v - a <= 0
     if (an < tmath::kAMin) an = tmath::kAMin;                    // (comparisons: a NaN passes through, tramp/base.py:252)
     if (an > tmath::kAMax) an = tmath::kAMax;
-    if (q.scal) q.scal[b] = LkScal{az, ax, an, lik1};
-    if (q.v_out) q.v_out[b] = v;
-    if (q.n_eff_out) q.n_eff_out[b] = se / q.V;
-    if (q.a_new_out) q.a_new_out[b] = q.damping != 0.0 ? q.damping * q.a_old[b] + (1.0 - q.damping) * an : an;
+    const LkScal c{az, ax, an, lik1};
+    if (write && threadIdx.x == 0) {
+        if (q.scal) q.scal[b] = c;
+        if (q.v_out) q.v_out[b] = v;
+        if (q.n_eff_out) q.n_eff_out[b] = se / q.V;
+        if (q.a_new_out) q.a_new_out[b] = q.damping != 0.0 ? q.damping * q.a_old[b] + (1.0 - q.damping) * an : an;
+    }
+    return c;
 }
 
-__global__ __launch_bounds__(kBlock) void lookup_scalars_kernel(LkScalArgs q) { lk_scalars(q, blockIdx.x); }
+__global__ __launch_bounds__(kBlock) void lookup_scalars_kernel(LkScalArgs q) { (void)lk_scalars(q, blockIdx.x, true); }
 
 // ---------------------------------------------------------------- rows in 16-byte pieces
 // A row of D elements is walked by LPR = min(64, 2^ceil(log2(D / N))) lanes, one 16-byte piece (N elements) per lane, in
@@ -277,6 +281,7 @@ __global__ __launch_bounds__(kBlock) void lookup_apply1_kernel(size_t V, size_t 
 // message to 10^6 positions of 64 columns 136 against 104 us), 4 make longer runs of every kind (89 and 103 us).
 constexpr int kKeep = 8;
 
+
 struct LkArgs {
     const int* off;
     const int* perm;
@@ -292,8 +297,9 @@ struct LkArgs {
     double s;
 };
 
-// what is made of the sum of a run: the gradient, the message to the table, the message to its positions, scale times the mean
-enum { LK_GRAD = 0, LK_BWD = 1, LK_FWD = 2, LK_MEAN = 3 };
+// what is made of the sum of a run: the gradient, the message to the table, the message to its positions, scale times the mean,
+// the row's share of the log-partition
+enum { LK_GRAD = 0, LK_BWD = 1, LK_FWD = 2, LK_MEAN = 3, LK_LOGZ = 4 };
 
 // rows perm[j0 + sub], perm[j0 + sub + S], ... of the run [j0, j0 + c), S = 1 << ls: added into acc, kept if KEEP (c <= kKeep S)
 template <typename T, int ROW, bool KEEP, bool ONCE>
@@ -416,7 +422,7 @@ __global__ __launch_bounds__(kBlock) void lookup_chunks_kernel(LkArgs a, LkScalA
     __shared__ double sm[kBlock / kWave][kWave][N];
     const size_t b = blockIdx.y;
     if (blockIdx.x == a.n_chunks * a.tiles) {
-        lk_scalars(q, b);
+        (void)lk_scalars(q, b, true);
         return;
     }
     const unsigned blk = blockIdx.x / a.tiles;
@@ -437,8 +443,8 @@ __global__ __launch_bounds__(kBlock) void lookup_chunks_kernel(LkArgs a, LkScalA
 }
 
 // Second launch: every run.  Workgroups, in this order: joins of the partial sums, block runs, wave runs, light ones.
-template <typename T, int ROW, int MODE>
-__global__ __launch_bounds__(kBlock) void lookup_rows_kernel(LkArgs a, const LkScal* __restrict__ scal, const T* __restrict__ bz,
+template <typename T, int ROW, int MODE, bool SELF>
+__global__ __launch_bounds__(kBlock) void lookup_rows_kernel(LkArgs a, LkScalArgs q, const LkScal* __restrict__ scal, const T* __restrict__ bz,
                                                              const T* __restrict__ x, double damping, const T* b_old, T* out,
                                                              T* __restrict__ r_out, const double* __restrict__ partials,
                                                              double* __restrict__ sr_ws) {
@@ -450,7 +456,7 @@ __global__ __launch_bounds__(kBlock) void lookup_rows_kernel(LkArgs a, const LkS
     unsigned blk = place.blk;
     const LkLane k = lk_lane<T>(a.lw, place.tile, a.D);
     LkScal c{};
-    if (MODE != LK_GRAD) c = scal[b];
+    if (MODE != LK_GRAD) c = SELF ? lk_scalars(q, b, place.blk == 0 && place.tile == 0) : scal[b];
     const T* xb = x + b * a.T * a.D;
     const bool act = k.valid > 0;
     double acc[N];
@@ -507,6 +513,23 @@ __global__ __launch_bounds__(kBlock) void lookup_rows_kernel(LkArgs a, const LkS
         if (act) lk_gather<T, ROW, true, true>(a, xb, k, j0, count, sub, ls, acc, pj, rows);
         if (ls) lk_wave_join<N>(a.lw, acc);
     }
+    if (MODE == LK_LOGZ) {
+        // 1/2 sum (bz + g)^2 / prec + D/2 log(2 pi / prec) over this column tile of the row
+        double h = 0.0;
+        if (act) {
+            T z[N];
+            lk_load<T, ROW>(bz + (b * a.V + (size_t)v) * a.D + k.col, k.valid, z);
+            const double prec = c.az + c.lik1 * (double)count, lg = 0.5 * log(2.0 * tmath::kPi / prec);
+#pragma unroll
+            for (int e = 0; e < N; ++e) {
+                const double t = (double)z[e] + a.s * acc[e];
+                if (e < k.valid) h += 0.5 * (t * t / prec) + lg;
+            }
+        }
+        for (int off = (1 << a.lw) >> 1; off; off >>= 1) h += __shfl_xor(h, off, 64);
+        if (first && k.l == 0) sr_ws[(b * a.V + (size_t)v) * a.tiles + place.tile] = h;
+        return;
+    }
     if (!act) return;
     if (MODE == LK_GRAD || MODE == LK_BWD) {
         if (first) lk_row_out<T, ROW, MODE>(a, c, k, b, v, count, acc, bz, damping, b_old, out, r_out);
@@ -528,7 +551,8 @@ __global__ __launch_bounds__(kBlock) void lookup_rows_kernel(LkArgs a, const LkS
         if (i < cnt) lk_position_out<T, ROW>(a, c.ax + c.an, k, b, (size_t)pj[i], sr, rows[i], damping, b_old, out, r_out);
 }
 
-// Third launch of the message to the positions: those of the heavy runs and the padded ones (slot -1: rx = 0)
+// Third launch of the message to the positions: those of the heavy runs and the padded ones (slot -1: rx = 0), the chunks that were
+// summed last first - they are the likeliest to be cached still (10^6 x 64 f32: 150 us forwards, 138 us backwards).
 template <typename T, int ROW>
 __global__ __launch_bounds__(kBlock) void lookup_spread_kernel(LkArgs a, const LkItem* __restrict__ spreads, const LkScal* __restrict__ scal,
                                                                const double* __restrict__ sr_ws, const T* __restrict__ bx, double damping,
@@ -538,7 +562,7 @@ __global__ __launch_bounds__(kBlock) void lookup_spread_kernel(LkArgs a, const L
     const unsigned blk = blockIdx.x / a.tiles;
     const LkLane k = lk_lane<T>(a.lw, blockIdx.x - blk * a.tiles, a.D);
     if (k.valid <= 0) return;
-    const LkItem it = spreads[blk];
+    const LkItem it = spreads[gridDim.x / a.tiles - 1 - blk];
     const double asum = scal[b].ax + scal[b].an;
     double sr[N];
 #pragma unroll
@@ -552,7 +576,7 @@ __global__ __launch_bounds__(kBlock) void lookup_spread_kernel(LkArgs a, const L
         for (int i = 0; i < UR; ++i) t[i] = j + i * G < it.end ? a.perm[j + i * G] : -1;
 #pragma unroll
         for (int i = 0; i < UR; ++i)
-            if (t[i] >= 0) lk_load<T, ROW>(bx + (b * a.T + (size_t)t[i]) * a.D + k.col, k.valid, v[i]);
+            if (t[i] >= 0) lk_load<T, ROW, true>(bx + (b * a.T + (size_t)t[i]) * a.D + k.col, k.valid, v[i]);
 #pragma unroll
         for (int i = 0; i < UR; ++i)
             if (t[i] >= 0) lk_position_out<T, ROW>(a, asum, k, b, (size_t)t[i], sr, v[i], damping, b_old, out, r_out);
@@ -644,34 +668,14 @@ __global__ __launch_bounds__(kBlock) void lookup_positions1_kernel(LkArgs a, con
 }
 
 // ---------------------------------------------------------------- log-partition
-// A = 1/2 sum_v (bz + g)^2 / prec + D/2 sum_v log(2 pi / prec)   (linear_channel.py:127-132)
-template <typename T>
-__global__ __launch_bounds__(kBlock) void lookup_logz_kernel(size_t V, size_t D, size_t Tn, double s, const int* __restrict__ off,
-                                                             const int* __restrict__ perm, const double* __restrict__ az_d,
-                                                             const double* __restrict__ ax_d, const T* __restrict__ bz,
-                                                             const T* __restrict__ x, double* __restrict__ partials) {
+// A = 1/2 sum_v (bz + g)^2 / prec + D/2 sum_v log(2 pi / prec)   (linear_channel.py:127-132): the rows' shares, added in two steps
+__global__ __launch_bounds__(kBlock) void lookup_fold_kernel(size_t n, const double* __restrict__ in, double* __restrict__ out) {
     __shared__ double smem[kBlock / kWave];
-    const size_t b = blockIdx.y, n = V * D;
-    const double az = az_d[b], lik1 = ax_d[b] * s * s;
+    const size_t b = blockIdx.y;
     double acc = 0.0;
-    for (size_t i = (size_t)blockIdx.x * kBlock + threadIdx.x; i < n; i += (size_t)gridDim.x * kBlock) {
-        const size_t v = i / D, d = i - v * D;
-        const int j0 = off[v], j1 = off[v + 1];
-        double g = 0.0;
-        for (int j = j0; j < j1; ++j) g += (double)x[(b * Tn + (size_t)perm[j]) * D + d];
-        const double prec = az + lik1 * (double)(j1 - j0), h = (double)bz[b * n + i] + s * g;
-        acc += 0.5 * (h * h / prec) + 0.5 * log(2.0 * tmath::kPi / prec);
-    }
+    for (size_t i = (size_t)blockIdx.x * kBlock + threadIdx.x; i < n; i += (size_t)gridDim.x * kBlock) acc += in[b * n + i];
     acc = block_sum(acc, smem);
-    if (threadIdx.x == 0) partials[b * gridDim.x + blockIdx.x] = acc;
-}
-
-__global__ __launch_bounds__(kBlock) void lookup_fold_kernel(int n, const double* __restrict__ partials, double* __restrict__ out) {
-    __shared__ double smem[kBlock / kWave];
-    double acc = 0.0;
-    for (int i = threadIdx.x; i < n; i += kBlock) acc += partials[(size_t)blockIdx.x * n + i];
-    acc = block_sum(acc, smem);
-    if (threadIdx.x == 0) out[blockIdx.x] = acc;
+    if (threadIdx.x == 0) out[b * gridDim.x + blockIdx.x] = acc;
 }
 
 // ---------------------------------------------------------------- handle
@@ -705,7 +709,7 @@ extern "C" int tramp_lookup_create(tramp_ctx* ctx, int dtype, size_t n_rows, siz
         while (lw < 6 && ((size_t)1 << lw) < pieces) ++lw;
         const size_t tiles = (pieces + ((size_t)1 << lw) - 1) >> lw;
         const int per_wave = kKeep << (6 - lw), per_block = kKeep << (8 - lw);
-        const bool by_position = n_cols * e < 64;
+        const bool short_rows = n_cols * e < 64;
         std::vector<LkItem> chunks, runs, joins, spreads;
         std::vector<int> waves, light, single, idx, code;
         for (size_t v = 0; v < n_rows; ++v) {
@@ -736,7 +740,7 @@ extern "C" int tramp_lookup_create(tramp_ctx* ctx, int dtype, size_t n_rows, siz
         const size_t n_light2 = light.size();
         light.insert(light.end(), single.begin(), single.end());
         size_t n_multi = 0;
-        if (by_position) {
+        if (short_rows) {
             idx.assign(n_rows, -1);
             for (size_t v = 0; v < n_rows; ++v)
                 if (counts[v] > 1) idx[v] = (int)n_multi++;
@@ -817,7 +821,7 @@ extern "C" int tramp_lookup_create(tramp_ctx* ctx, int dtype, size_t n_rows, siz
         lk->lw = lw;
         lk->tiles = (unsigned)tiles;
         lk->row = n_cols % piece ? LK_TAIL : n_cols * e % 128 ? LK_WHOLE : LK_LINES;
-        lk->by_position = by_position;
+        lk->short_rows = short_rows;
         *out = lk;
         return TRAMP_OK;
     } catch (const std::exception&) {
@@ -837,6 +841,12 @@ extern "C" int tramp_lookup_destroy(tramp_ctx* ctx, tramp_lookup* lk) {
     if (!ctx) return TRAMP_EINVAL;                           \
     TRAMP_REQUIRE(ctx, lk && lk->device == ctx->device);     \
     TRAMP_REQUIRE(ctx, batch <= 65535)
+
+// do the rows of x and y (bytes each) share memory?
+static bool lk_overlap(const void* x, size_t nx, const void* y, size_t ny) {
+    const uintptr_t a = (uintptr_t)x, b = (uintptr_t)y;
+    return x && y && a < b + ny && b < a + nx;
+}
 
 // CALL(ROW) for the handle's kind of rows
 #define LK_BY_ROW(lk, CALL)               \
@@ -880,7 +890,9 @@ static int lookup_apply(tramp_ctx* ctx, const tramp_lookup* lk, size_t batch, co
 
 extern "C" int tramp_lookup_apply(tramp_ctx* ctx, tramp_lookup* lk, size_t batch, const void* z_d, void* x_d) {
     LK_REQUIRE_CALL(ctx, lk, batch);
-    TRAMP_REQUIRE(ctx, z_d && x_d && z_d != x_d);
+    TRAMP_REQUIRE(ctx, z_d && x_d);
+    const size_t row = batch * lk->D * dtype_size(lk->dtype);
+    TRAMP_REQUIRE(ctx, !lk_overlap(z_d, lk->V * row, x_d, lk->T * row));
     if (!batch) return TRAMP_OK;
     return lk->dtype == TRAMP_F64 ? lookup_apply<double>(ctx, lk, batch, (const double*)z_d, (double*)x_d)
                                   : lookup_apply<float>(ctx, lk, batch, (const float*)z_d, (float*)x_d);
@@ -902,15 +914,22 @@ static LkScalArgs lk_scal_args(const tramp_lookup* lk, int dir, const double* az
     return q;
 }
 
-// ctx->ws of a call: [scalars | partial sums | scale r of the heavy runs, or of all runs of two and more positions]
+// ctx->ws of a call: [scalars | partial sums | scale r of the heavy runs, or of all runs of two and more positions, or the
+// shares of the log-partition]
 struct LkWs {
     LkScal* scal;
     double* partials;
     double* sr;
 };
-static int lk_workspace(tramp_ctx* ctx, const tramp_lookup* lk, size_t batch, bool forward, LkWs* w) {
+// Short rows in the order of the positions: one column from 4 MB of positions on (10^6 f64 44 -> 33 us, 16 x 60000 29 -> 22 us;
+// 64 x 2000 would be 10.0 against 8.3 us, the price of the second launch), more columns where heavy runs take launches of
+// their own anyway (10^6 x 7 f64 83 -> 63 us; 8 x 60000 x 4 f64 without any 19.5 against 23.7 us).
+static bool lk_by_position(const tramp_lookup* lk, size_t batch) {
+    return lk->short_rows && batch * lk->T * lk->D * dtype_size(lk->dtype) >= ((size_t)4 << 20) && (lk->D == 1 || lk->n_chunks);
+}
+static int lk_workspace(tramp_ctx* ctx, const tramp_lookup* lk, size_t batch, size_t n_extra, LkWs* w) {
     const size_t n_scal = (batch * sizeof(LkScal) + 255) & ~(size_t)255, n_part = batch * lk->n_chunks * lk->D * sizeof(double);
-    const size_t n_sr = !forward ? 0 : batch * (lk->by_position ? lk->n_multi : lk->n_joins) * lk->D * sizeof(double);
+    const size_t n_sr = n_extra * sizeof(double);
     int rc = tramp_ws_reserve(ctx, n_scal + n_part + n_sr);
     if (rc) return rc;
     char* m = reinterpret_cast<char*>(ctx->ws);
@@ -948,14 +967,22 @@ static int launch_rows(tramp_ctx* ctx, const tramp_lookup* lk, size_t batch, con
     const size_t blocks = (size_t)a.n_joins + a.n_runs + a.wave_blocks + ((size_t)a.n_light + G - 1) / G;
     TRAMP_REQUIRE(ctx, blocks * lk->tiles < 0x7fffffffu && (size_t)lk->n_spreads * lk->tiles < 0x7fffffffu &&
                            (size_t)lk->n_chunks * lk->tiles < 0x7ffffffeu);
-    if (lk->n_chunks || q)
-        hipLaunchKernelGGL((lookup_chunks_kernel<T, ROW, MODE != LK_FWD && MODE != LK_MEAN>), dim3(lk->n_chunks * lk->tiles + (q ? 1 : 0), (unsigned)batch),
-                           dim3(kBlock), 0, ctx->stream, a, q ? *q : LkScalArgs{}, x, w.partials);
     a.blocks = (unsigned)blocks;
     a.spread = lk_spread(batch, blocks * lk->tiles);
-    if (blocks)
-        hipLaunchKernelGGL((lookup_rows_kernel<T, ROW, MODE>), lk_grid(batch, blocks * lk->tiles, a.spread), dim3(kBlock), 0, ctx->stream, a,
-                           w.scal, bz, x, damping, b_old, out, r_out, w.partials, w.sr);
+    // few workgroups and few counts: each makes the scalars for itself, one launch less (V = 1000, 2000 positions 10.2 -> 7.6 us;
+    // with up to 4096 workgroups 8 x 60000 x 8 f64 would be 31.5 against 27.1 us)
+    const bool self = q && !lk->n_chunks && blocks && blocks * lk->tiles * batch <= 1024 && lk->K <= 4 * kBlock && q->a_new_out != q->az &&
+                      q->a_new_out != q->ax;
+    if (lk->n_chunks || (q && !self))
+        hipLaunchKernelGGL((lookup_chunks_kernel<T, ROW, MODE != LK_FWD && MODE != LK_MEAN>), dim3(lk->n_chunks * lk->tiles + (q ? 1 : 0), (unsigned)batch),
+                           dim3(kBlock), 0, ctx->stream, a, q ? *q : LkScalArgs{}, x, w.partials);
+    const dim3 grid = lk_grid(batch, blocks * lk->tiles, a.spread);
+    if (MODE != LK_GRAD && self)
+        hipLaunchKernelGGL((lookup_rows_kernel<T, ROW, MODE, MODE != LK_GRAD>), grid, dim3(kBlock), 0, ctx->stream, a, *q, w.scal, bz, x, damping,
+                           b_old, out, r_out, w.partials, w.sr);
+    else if (blocks)
+        hipLaunchKernelGGL((lookup_rows_kernel<T, ROW, MODE, false>), grid, dim3(kBlock), 0, ctx->stream, a, LkScalArgs{}, w.scal, bz, x, damping,
+                           b_old, out, r_out, w.partials, w.sr);
     if (MODE == LK_FWD && lk->n_spreads)
         hipLaunchKernelGGL((lookup_spread_kernel<T, ROW>), dim3(lk->n_spreads * lk->tiles, (unsigned)batch), dim3(kBlock), 0, ctx->stream, a,
                            lk->spreads, w.scal, w.sr, x, damping, b_old, out, r_out);
@@ -984,10 +1011,12 @@ static int run_rows(tramp_ctx* ctx, const tramp_lookup* lk, size_t batch, const 
 
 extern "C" int tramp_lookup_gradient(tramp_ctx* ctx, tramp_lookup* lk, size_t batch, const void* x_d, void* g_d) {
     LK_REQUIRE_CALL(ctx, lk, batch);
-    TRAMP_REQUIRE(ctx, x_d && g_d && x_d != g_d);
+    TRAMP_REQUIRE(ctx, x_d && g_d);
+    const size_t row = batch * lk->D * dtype_size(lk->dtype);
+    TRAMP_REQUIRE(ctx, !lk_overlap(g_d, lk->V * row, x_d, lk->T * row));
     if (!batch) return TRAMP_OK;
     LkWs w;
-    int rc = lk_workspace(ctx, lk, batch, false, &w);
+    int rc = lk_workspace(ctx, lk, batch, 0, &w);
     if (rc) return rc;
     if (lk->dtype == TRAMP_F64)
         return run_rows<double, LK_GRAD>(ctx, lk, batch, w, nullptr, nullptr, (const double*)x_d, 0.0, nullptr, (double*)g_d, nullptr);
@@ -1013,14 +1042,15 @@ static int lookup_message(tramp_ctx* ctx, tramp_lookup* lk, int dir, size_t batc
                           const double* ax_d, const T* bx, double damping, const double* a_old_d, const T* b_old, double* a_new_d,
                           T* b_new, T* r_d, double* v_d) {
     LkWs w;
-    int rc = lk_workspace(ctx, lk, batch, dir == TRAMP_FWD, &w);
+    const bool by_position = dir == TRAMP_FWD && lk_by_position(lk, batch);
+    int rc = lk_workspace(ctx, lk, batch, dir == TRAMP_BWD ? 0 : batch * (by_position ? lk->n_multi : lk->n_joins) * lk->D, &w);
     if (rc) return rc;
     LkScalArgs q = lk_scal_args(lk, dir, az_d, ax_d, damping, a_old_d);
     q.scal = w.scal;
     q.v_out = v_d;
     q.a_new_out = a_new_d;
     if (dir == TRAMP_BWD) return run_rows<T, LK_BWD>(ctx, lk, batch, w, &q, bz, bx, damping, b_old, b_new, r_d);
-    if (lk->by_position) return run_rows<T, LK_MEAN>(ctx, lk, batch, w, &q, bz, bx, damping, b_old, b_new, r_d);
+    if (by_position) return run_rows<T, LK_MEAN>(ctx, lk, batch, w, &q, bz, bx, damping, b_old, b_new, r_d);
     return run_rows<T, LK_FWD>(ctx, lk, batch, w, &q, bz, bx, damping, b_old, b_new, r_d);
 }
 
@@ -1029,7 +1059,10 @@ extern "C" int tramp_lookup_message(tramp_ctx* ctx, tramp_lookup* lk, int dir, s
                                     const void* b_old_d, double* a_new_d, void* b_new_d, void* r_d, double* v_d) {
     LK_REQUIRE_CALL(ctx, lk, batch);
     TRAMP_REQUIRE(ctx, (dir == TRAMP_FWD || dir == TRAMP_BWD) && az_d && bz_d && ax_d && bx_d && a_new_d && b_new_d);
-    TRAMP_REQUIRE(ctx, b_new_d != bz_d && b_new_d != bx_d);
+    const size_t row = batch * lk->D * dtype_size(lk->dtype), nz = lk->V * row, nx = lk->T * row, no = dir == TRAMP_FWD ? nx : nz;
+    TRAMP_REQUIRE(ctx, !lk_overlap(b_new_d, no, bz_d, nz) && !lk_overlap(b_new_d, no, bx_d, nx));
+    TRAMP_REQUIRE(ctx, !lk_overlap(r_d, no, bz_d, nz) && !lk_overlap(r_d, no, bx_d, nx) && !lk_overlap(r_d, no, b_new_d, no));
+    TRAMP_REQUIRE(ctx, damping == 0.0 || b_old_d == b_new_d || !lk_overlap(b_old_d, no, b_new_d, no));
     TRAMP_REQUIRE(ctx, damping == 0.0 || (a_old_d && b_old_d));
     if (!batch) return TRAMP_OK;
     if (lk->dtype == TRAMP_F64)
@@ -1044,17 +1077,19 @@ extern "C" int tramp_lookup_log_partition(tramp_ctx* ctx, tramp_lookup* lk, size
     LK_REQUIRE_CALL(ctx, lk, batch);
     TRAMP_REQUIRE(ctx, az_d && bz_d && ax_d && bx_d && out_d);
     if (!batch) return TRAMP_OK;
-    const int nblk = blocks_for(lk->V * lk->D, 1);
-    int rc = tramp_ws_reserve(ctx, batch * (size_t)nblk * sizeof(double));
+    const size_t n = lk->V * lk->tiles;
+    const int nblk = blocks_for(n, 1);
+    LkWs w;
+    int rc = lk_workspace(ctx, lk, batch, batch * (n + (size_t)nblk), &w);
     if (rc) return rc;
-    dim3 grid(nblk, (unsigned)batch);
-    if (lk->dtype == TRAMP_F64)
-        hipLaunchKernelGGL((lookup_logz_kernel<double>), grid, dim3(kBlock), 0, ctx->stream, lk->V, lk->D, lk->T, lk->s, lk->off,
-                           lk->perm, az_d, ax_d, (const double*)bz_d, (const double*)bx_d, ctx->ws);
-    else
-        hipLaunchKernelGGL((lookup_logz_kernel<float>), grid, dim3(kBlock), 0, ctx->stream, lk->V, lk->D, lk->T, lk->s, lk->off,
-                           lk->perm, az_d, ax_d, (const float*)bz_d, (const float*)bx_d, ctx->ws);
-    hipLaunchKernelGGL(lookup_fold_kernel, dim3((unsigned)batch), dim3(kBlock), 0, ctx->stream, nblk, ctx->ws, out_d);
+    LkScalArgs q = lk_scal_args(lk, TRAMP_FWD, az_d, ax_d, 0.0, nullptr);
+    q.scal = w.scal;
+    rc = lk->dtype == TRAMP_F64
+             ? run_rows<double, LK_LOGZ>(ctx, lk, batch, w, &q, (const double*)bz_d, (const double*)bx_d, 0.0, nullptr, nullptr, nullptr)
+             : run_rows<float, LK_LOGZ>(ctx, lk, batch, w, &q, (const float*)bz_d, (const float*)bx_d, 0.0, nullptr, nullptr, nullptr);
+    if (rc) return rc;
+    hipLaunchKernelGGL(lookup_fold_kernel, dim3(nblk, (unsigned)batch), dim3(kBlock), 0, ctx->stream, n, w.sr, w.sr + batch * n);
+    hipLaunchKernelGGL(lookup_fold_kernel, dim3(1, (unsigned)batch), dim3(kBlock), 0, ctx->stream, (size_t)nblk, w.sr + batch * n, out_d);
     TRAMP_LAUNCH_CHECK(ctx);
     return TRAMP_OK;
 }
