@@ -1552,12 +1552,12 @@ class LookupChannel(Channel):
         arg._one = h.ndim == nd
         return arg
 
-    def _out(self, out, batch, n, dtype):
-        "the caller's result buffer, checked, or a new one"
+    def _out(self, out, shape, dtype):
+        "the caller's buffer, checked, or a new one"
         if out is None:
-            return self.ctx.empty((batch, n), dtype)
-        if not isinstance(out, DeviceArray) or out.ctx is not self.ctx or out.dtype != np.dtype(dtype) or out.size != batch * n:
-            raise ValueError(f"the result needs a device array of {batch} x {n} {np.dtype(dtype)} in this context, got {out!r}")
+            return self.ctx.empty(shape, dtype)
+        if not isinstance(out, DeviceArray) or out.ctx is not self.ctx or out.dtype != np.dtype(dtype) or out.size != int(np.prod(shape)):
+            raise ValueError(f"expected a device array of {shape} {np.dtype(dtype)} in this context, got {out!r}")
         return out
 
     _ret = staticmethod(ConvChannel._ret)
@@ -1566,7 +1566,7 @@ class LookupChannel(Channel):
     def _linear(self, entry, src, x_side, out):
         v = self._vec(src, x_side)
         full, n = (self._zshape, self.Nz) if x_side else (self._xshape, self.Nx)
-        dev = self._out(out, v.batch, n, self.dtype)
+        dev = self._out(out, (v.batch, n), self.dtype)
         self.ctx._call(entry, self._handle, v.batch, v.dev.ptr, dev.ptr)
         if out is not None or not v.was_host:
             return dev
@@ -1621,14 +1621,15 @@ class LookupChannel(Channel):
         ctx = self.ctx
         z, x, a_z, a_x = self._args(az, bz, ax, bx)
         tgt, a_t = (x, a_x) if direction == _lib.FWD else (z, a_z)
-        a_new, b_new = self._out(out_a, z.batch, 1, np.float64), self._out(out_b, z.batch, tgt.n, self.dtype)
+        a_shape, b_shape = (z.batch,), (z.batch, tgt.n)
+        a_new, b_new = self._out(out_a, a_shape, np.float64), self._out(out_b, b_shape, self.dtype)
         if damping:
             if old_a is None or old_b is None:
                 raise ValueError("damping needs old_a and old_b")
-            self._out(old_a, z.batch, 1, np.float64)
-            self._out(old_b, z.batch, tgt.n, self.dtype)
-        r = ctx.empty((z.batch, tgt.n), self.dtype) if want_posterior else None
-        v = ctx.empty((z.batch,), np.float64) if want_posterior else None
+            self._out(old_a, a_shape, np.float64)
+            self._out(old_b, b_shape, self.dtype)
+        r = ctx.empty(b_shape, self.dtype) if want_posterior else None
+        v = ctx.empty(a_shape, np.float64) if want_posterior else None
         ctx._call("tramp_lookup_message", self._handle, direction, z.batch, a_z.dev.ptr, z.dev.ptr, a_x.dev.ptr, x.dev.ptr,
                   float(damping or 0.0), old_a.ptr if old_a is not None else None, old_b.ptr if old_b is not None else None,
                   a_new.ptr, b_new.ptr, r.ptr if r is not None else None, v.ptr if v is not None else None)
