@@ -106,10 +106,16 @@ def test_messages(ctx, shape, direction, dtype):
         assert abs(DA[i] - (0.3 * a0[i] + 0.7 * ra)) <= 2 * rel_a * (a0[i] + ra)
         want = 0.3 * b0[i].astype(float) + 0.7 * rb
         assert (np.abs(DB[i] - want) <= eps2(dtype) * np.abs(want) + k * (mag + np.abs(b0[i]))).all()
+        # r = (z + g) / prec: c additions, a product with s, a sum, a quotient (as a product with 1 / prec) and the product with s,
+        # each off by u of its magnitude, which (|z| + |g|) / prec bounds.  (Not |b'|'s magnitude over a + a': that of a row nobody
+        # reads is |z| a' / az, far below |r| (az + a').)
         mean = ref.mean(az[i], z[i], ax[i], x[i])
+        size = (np.abs(z[i].astype(float)).reshape(ref.V, ref.D) + abs(ref.s) * LookupFactor(ref.tok, ref.V, ref.D, 1.0).gradient(
+            np.abs(x[i].astype(float)))) / ref._prec(az[i], ax[i])[:, None]
         if direction == "forward":
-            mean = np.where(ref.tok[:, None] >= 0, ref.s * mean[np.maximum(ref.tok, 0)], 0.0)
-        lim = k * mag / ((ax[i] if direction == "forward" else az[i]) + ra)   # mag holds |r| (a + a')
+            at = np.maximum(ref.tok, 0)
+            mean, size = (np.where(ref.tok[:, None] >= 0, abs(ref.s) * q[at], 0.0) for q in (mean * np.sign(ref.s), size))
+        lim = 2 * (ref.count.max() + 8) * U * size.reshape(-1)
         assert (np.abs(R[i] - mean.reshape(-1)) <= eps2(dtype) * np.abs(mean.reshape(-1)) + lim).all()
         v = float(getattr(ref, direction + "_variance")(az[i], ax[i]))
         assert abs(Vv[i] - v) <= rel_a * v

@@ -1556,7 +1556,8 @@ class LookupChannel(Channel):
         "the caller's buffer, checked, or a new one"
         if out is None:
             return self.ctx.empty(shape, dtype)
-        if not isinstance(out, DeviceArray) or out.ctx is not self.ctx or out.dtype != np.dtype(dtype) or out.size != int(np.prod(shape)):
+        n = shape[0] if len(shape) == 1 else shape[0] * shape[1]
+        if not isinstance(out, DeviceArray) or out.ctx is not self.ctx or out.dtype != dtype or out.size != n:
             raise ValueError(f"expected a device array of {shape} {np.dtype(dtype)} in this context, got {out!r}")
         return out
 

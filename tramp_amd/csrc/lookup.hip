@@ -22,10 +22,11 @@
 
 #include <algorithm>
 #include <new>
+#include <type_traits>
 #include <vector>
 
 struct LkItem {
-    int token, start, end, slot;      // positions perm[start .. end); slot: of the partial sum, or the index of the heavy run
+    int token, start, end, slot;      // positions perm[start .. end); slot: by list (tramp_lookup)
 };
 
 struct tramp_lookup {
@@ -43,8 +44,8 @@ struct tramp_lookup {
     const LkItem* joins;         // {token, first chunk, one behind the last, index}
     const LkItem* spreads;       // the chunks' positions and the padded ones
     const LkItem* runs;          // runs for one workgroup
-    const int* waves;            // tokens of the runs for one wave
-    const int* light;            // tokens of the shorter runs, those of one position last
+    const LkItem* waves;         // runs for one wave
+    const LkItem* light;         // the shorter runs, by falling length; slot: the first position
     const int* idx;              // [V] place among the runs of two and more positions (short rows only)
     const int* code;             // [T] that place, -1 where padded, -2 - token where the run is this position (short rows only)
     int K;
@@ -288,8 +289,8 @@ struct LkArgs {
     const LkItem* chunks;
     const LkItem* joins;
     const LkItem* runs;
-    const int* waves;
-    const int* light;            // null: all rows of the table (those of the kinds above left out)
+    const LkItem* waves;
+    const LkItem* light;         // null: all rows of the table (those of the kinds above left out)
     const int* idx;
     size_t V, D, T;
     unsigned n_chunks, n_joins, n_runs, n_waves, wave_blocks, n_light, n_multi, blocks, tiles, batch;
@@ -301,29 +302,30 @@ struct LkArgs {
 // the row's share of the log-partition
 enum { LK_GRAD = 0, LK_BWD = 1, LK_FWD = 2, LK_MEAN = 3, LK_LOGZ = 4 };
 
-// rows perm[j0 + sub], perm[j0 + sub + S], ... of the run [j0, j0 + c), S = 1 << ls: added into acc, kept if KEEP (c <= kKeep S)
-template <typename T, int ROW, bool KEEP, bool ONCE>
-__device__ __forceinline__ void lk_gather(const LkArgs& a, const T* __restrict__ xb, const LkLane& k, int j0, int c, int sub, int ls,
-                                          double (&acc)[LkVec<T>::N], int (&pj)[kKeep], T (&rows)[kKeep][LkVec<T>::N]) {
-    constexpr int N = LkVec<T>::N;
+// rows perm[j0 + sub], perm[j0 + sub + S], ... of the run [j0, j0 + c), S = 1 << ls: added into acc, C in flight; KEEP: there are
+// at most C and they stay in `rows`.  p0: the position of a run of one, if known.
+template <typename T, int ROW, int C, bool KEEP, bool ONCE>
+__device__ __forceinline__ void lk_gather(const LkArgs& a, const T* __restrict__ xb, const LkLane& k, int j0, int c, int sub, int ls, int p0,
+                                          double (&acc)[LkVec<T>::N], int (&pj)[C], T (&rows)[C][LkVec<T>::N]) {
+    constexpr int N = LkVec<T>::N, Q = C < 4 ? C : 4;
     const int cnt = c > sub ? ((c - sub - 1) >> ls) + 1 : 0;
     const int* pp = a.perm + j0 + sub;
-    for (int base = 0; base < cnt; base += kKeep) {
+    for (int base = 0; base < cnt; base += C) {
 #pragma unroll
-        for (int q = 0; q < kKeep; q += 4)
+        for (int q = 0; q < C; q += Q)
             if (base + q < cnt) {
 #pragma unroll
-                for (int i = q; i < q + 4; ++i) pj[i] = base + i < cnt ? pp[(size_t)(base + i) << ls] : -1;
+                for (int i = q; i < q + Q; ++i) pj[i] = i == 0 && c == 1 && p0 >= 0 ? p0 : base + i < cnt ? pp[(size_t)(base + i) << ls] : -1;
             }
 #pragma unroll
-        for (int q = 0; q < kKeep; q += 4)
+        for (int q = 0; q < C; q += Q)
             if (base + q < cnt) {
 #pragma unroll
-                for (int i = q; i < q + 4; ++i)
+                for (int i = q; i < q + Q; ++i)
                     if (base + i < cnt) lk_load<T, ROW, ONCE>(xb + (size_t)pj[i] * a.D + k.col, k.valid, rows[i]);
             }
 #pragma unroll
-        for (int i = 0; i < kKeep; ++i)
+        for (int i = 0; i < C; ++i)
             if (base + i < cnt) {
 #pragma unroll
                 for (int e = 0; e < N; ++e) acc[e] += (double)rows[i][e];
@@ -351,22 +353,10 @@ template <int N> __device__ __forceinline__ void lk_block_join(const LkLane& k, 
     for (int e = 0; e < N; ++e) acc[e] = ((sm[0][lane][e] + sm[1][lane][e]) + sm[2][lane][e]) + sm[3][lane][e];
 }
 
-// scale times the posterior mean of a row with the sum acc
-template <typename T, int ROW>
-__device__ __forceinline__ void lk_mean(const LkArgs& a, const LkScal& c, const LkLane& k, size_t b, int v, int count, const T* __restrict__ bz,
-                                        const double (&acc)[LkVec<T>::N], double (&sr)[LkVec<T>::N]) {
-    constexpr int N = LkVec<T>::N;
-    T z[N];
-    lk_load<T, ROW>(bz + (b * a.V + (size_t)v) * a.D + k.col, k.valid, z);
-    const double prec = c.az + c.lik1 * (double)count;
-#pragma unroll
-    for (int e = 0; e < N; ++e) sr[e] = a.s * (((double)z[e] + a.s * acc[e]) / prec);
-}
-
 // the gradient or the message to the table
 template <typename T, int ROW, int MODE>
 __device__ __forceinline__ void lk_row_out(const LkArgs& a, const LkScal& c, const LkLane& k, size_t b, int v, int count,
-                                           const double (&acc)[LkVec<T>::N], const T* __restrict__ bz, double damping, const T* b_old,
+                                           const double (&acc)[LkVec<T>::N], const T (&z)[LkVec<T>::N], double damping, const T* b_old,
                                            T* out, T* __restrict__ r_out) {
     constexpr int N = LkVec<T>::N;
     const size_t at = (b * a.V + (size_t)v) * a.D + k.col;
@@ -375,19 +365,22 @@ __device__ __forceinline__ void lk_row_out(const LkArgs& a, const LkScal& c, con
 #pragma unroll
         for (int e = 0; e < N; ++e) o[e] = T(a.s * acc[e]);
     } else {
-        const double lik = c.lik1 * (double)count, prec = c.az + lik;
-        T z[N], r[N], old[N];
-        lk_load<T, ROW, true>(bz + at, k.valid, z);
+        const double lik = c.lik1 * (double)count, inv = 1.0 / (c.az + lik);
+        const double mg = a.s * ((c.az + c.an) * inv), mz = (c.an - lik) * inv;
+        T old[N];
         if (damping != 0.0) lk_load<T, ROW>(b_old + at, k.valid, old);
 #pragma unroll
         for (int e = 0; e < N; ++e) {
-            const double g = a.s * acc[e];
-            double m = (g * (c.az + c.an) + (double)z[e] * (c.an - lik)) / prec;
+            double m = mg * acc[e] + mz * (double)z[e];
             if (damping != 0.0) m = damping * (double)old[e] + (1.0 - damping) * m;
             o[e] = T(m);
-            r[e] = T(((double)z[e] + g) / prec);
         }
-        if (r_out) lk_store<T, ROW>(r_out + at, k.valid, r);
+        if (r_out) {
+            T r[N];
+#pragma unroll
+            for (int e = 0; e < N; ++e) r[e] = T(((double)z[e] + a.s * acc[e]) * inv);
+            lk_store<T, ROW>(r_out + at, k.valid, r);
+        }
     }
     lk_store<T, ROW>(out + at, k.valid, o);
 }
@@ -433,7 +426,7 @@ __global__ __launch_bounds__(kBlock) void lookup_chunks_kernel(LkArgs a, LkScalA
     T rows[kKeep][N];
 #pragma unroll
     for (int e = 0; e < N; ++e) acc[e] = 0.0;
-    if (k.valid > 0) lk_gather<T, ROW, false, ONCE>(a, x + b * a.T * a.D, k, it.start, it.end - it.start, k.group, 8 - a.lw, acc, pj, rows);
+    if (k.valid > 0) lk_gather<T, ROW, kKeep, false, ONCE>(a, x + b * a.T * a.D, k, it.start, it.end - it.start, k.group, 8 - a.lw, -1, acc, pj, rows);
     lk_block_join<N>(k, acc, sm);
     if (threadIdx.x >= (1u << a.lw) || k.valid <= 0) return;
     double* p = partials + (b * a.n_chunks + (size_t)it.slot) * a.D + k.col;
@@ -461,14 +454,19 @@ __global__ __launch_bounds__(kBlock) void lookup_rows_kernel(LkArgs a, LkScalArg
     const bool act = k.valid > 0;
     double acc[N];
     int pj[kKeep];
-    T rows[kKeep][N];
+    T rows[kKeep][N], z[N];
 #pragma unroll
     for (int e = 0; e < N; ++e) acc[e] = 0.0;
-    int v, j0, count, sub, ls, place_ws = -1;
+    int v, j0, count, sub, ls, p0 = -1, place_ws = -1;
     bool first = true;
+    // the row of the table is asked for as soon as it is known, the sum comes later
+    const auto row_of = [&](int v) {
+        if (MODE != LK_GRAD && act) lk_load<T, ROW, MODE == LK_BWD>(bz + (b * a.V + (size_t)v) * a.D + k.col, k.valid, z);
+    };
     if (blk < a.n_joins) {
         const LkItem it = a.joins[blk];
         v = it.token;
+        row_of(v);
         count = a.off[v + 1] - a.off[v];
         const int G = kBlock >> a.lw;
         const double* p = partials + b * a.n_chunks * a.D + k.col;
@@ -484,46 +482,99 @@ __global__ __launch_bounds__(kBlock) void lookup_rows_kernel(LkArgs a, LkScalArg
     } else if ((blk -= a.n_joins) < a.n_runs) {
         const LkItem it = a.runs[blk];
         v = it.token;
+        row_of(v);
         j0 = it.start;
         count = it.end - it.start;
         sub = k.group;
         ls = 8 - a.lw;
         first = threadIdx.x < (1u << a.lw);
-        if (act) lk_gather<T, ROW, true, true>(a, xb, k, j0, count, sub, ls, acc, pj, rows);
+        if (act) lk_gather<T, ROW, kKeep, true, true>(a, xb, k, j0, count, sub, ls, p0, acc, pj, rows);
         lk_block_join<N>(k, acc, sm);
     } else {
         blk -= a.n_runs;
         if (blk < a.wave_blocks) {
             const unsigned w = blk * (kBlock / kWave) + (threadIdx.x >> 6);
             if (w >= a.n_waves) return;
-            v = a.waves[w];
+            const LkItem it = a.waves[w];
+            v = it.token;
+            row_of(v);
+            j0 = it.start;
+            count = it.end - it.start;
             sub = (threadIdx.x & 63) >> a.lw;
             ls = 6 - a.lw;
             first = (threadIdx.x & 63) < (1u << a.lw);
         } else {
             const size_t u = (size_t)(blk - a.wave_blocks) * (kBlock >> a.lw) + k.group;
             if (u >= a.n_light) return;
-            v = a.light ? a.light[u] : (int)u;
             sub = 0;
             ls = 0;
+            if (a.light) {
+                const LkItem it = a.light[u];
+                v = it.token;
+                row_of(v);
+                j0 = it.start;
+                count = it.end - it.start;
+                p0 = it.slot;
+            } else {
+                v = (int)u;
+                row_of(v);
+                j0 = a.off[v];
+                count = a.off[v + 1] - j0;
+            }
         }
-        j0 = a.off[v];
-        count = a.off[v + 1] - j0;
         if (ls == 0 && count > kKeep) return;                      // of another kind
-        if (act) lk_gather<T, ROW, true, true>(a, xb, k, j0, count, sub, ls, acc, pj, rows);
+        // Most runs are of one or two positions.  Where a row costs instructions rather than bytes a wave goes no deeper than its
+        // longest run (8 x 55612 positions of 78 f32 161 -> 155 us, 64 x 96196 of 6 f64 357 -> 320 us, gradient of 64 x 100000
+        // f64 92 -> 78 us); whole lines and long f64 rows are better off with one body (100000 x 21 f64 119 us against 125).
+        constexpr bool may = ROW == LK_TAIL || (ROW == LK_WHOLE && (MODE == LK_FWD || MODE == LK_MEAN));
+        const bool shallow = may && (sizeof(T) == 4 || a.lw <= 2);
+        if (shallow && MODE != LK_LOGZ && ls == 0 && !__any(count > 4)) {
+            const auto run = [&](auto depth) {
+                constexpr int C = decltype(depth)::value;
+                int qj[C];
+                T part[C][N];
+                lk_gather<T, ROW, C, true, true>(a, xb, k, j0, count, 0, 0, p0, acc, qj, part);
+                if (MODE == LK_GRAD || MODE == LK_BWD) {
+                    lk_row_out<T, ROW, MODE>(a, c, k, b, v, count, acc, z, damping, b_old, out, r_out);
+                    return;
+                }
+                double sr[N];
+                const double f = a.s / (c.az + c.lik1 * (double)count);
+#pragma unroll
+                for (int e = 0; e < N; ++e) sr[e] = f * ((double)z[e] + a.s * acc[e]);
+                if (MODE == LK_MEAN) {
+                    double* r = sr_ws + (b * a.n_multi + (size_t)a.idx[v]) * a.D + k.col;
+#pragma unroll
+                    for (int e = 0; e < N; ++e)
+                        if (e < k.valid) r[e] = sr[e];
+                    return;
+                }
+#pragma unroll
+                for (int i = 0; i < C; ++i)
+                    if (i < count) lk_position_out<T, ROW>(a, c.ax + c.an, k, b, (size_t)qj[i], sr, part[i], damping, b_old, out, r_out);
+            };
+            const bool two = __any(count > 1), four = __any(count > 2);
+            if (!act) return;
+            if (four)
+                run(std::integral_constant<int, 4>{});
+            else if (two)
+                run(std::integral_constant<int, 2>{});
+            else
+                run(std::integral_constant<int, 1>{});
+            return;
+        }
+        if (act) lk_gather<T, ROW, kKeep, true, true>(a, xb, k, j0, count, sub, ls, p0, acc, pj, rows);
         if (ls) lk_wave_join<N>(a.lw, acc);
     }
     if (MODE == LK_LOGZ) {
         // 1/2 sum (bz + g)^2 / prec + D/2 log(2 pi / prec) over this column tile of the row
         double h = 0.0;
         if (act) {
-            T z[N];
-            lk_load<T, ROW>(bz + (b * a.V + (size_t)v) * a.D + k.col, k.valid, z);
-            const double prec = c.az + c.lik1 * (double)count, lg = 0.5 * log(2.0 * tmath::kPi / prec);
+            const double prec = c.az + c.lik1 * (double)count, lg = 0.5 * log(2.0 * tmath::kPi / prec), half = 0.5 / prec;
 #pragma unroll
             for (int e = 0; e < N; ++e) {
                 const double t = (double)z[e] + a.s * acc[e];
-                if (e < k.valid) h += 0.5 * (t * t / prec) + lg;
+                if (e < k.valid) h += half * (t * t) + lg;
             }
         }
         for (int off = (1 << a.lw) >> 1; off; off >>= 1) h += __shfl_xor(h, off, 64);
@@ -532,11 +583,13 @@ __global__ __launch_bounds__(kBlock) void lookup_rows_kernel(LkArgs a, LkScalArg
     }
     if (!act) return;
     if (MODE == LK_GRAD || MODE == LK_BWD) {
-        if (first) lk_row_out<T, ROW, MODE>(a, c, k, b, v, count, acc, bz, damping, b_old, out, r_out);
+        if (first) lk_row_out<T, ROW, MODE>(a, c, k, b, v, count, acc, z, damping, b_old, out, r_out);
         return;
     }
     double sr[N];
-    lk_mean<T, ROW>(a, c, k, b, v, count, bz, acc, sr);
+    const double f = a.s / (c.az + c.lik1 * (double)count);
+#pragma unroll
+    for (int e = 0; e < N; ++e) sr[e] = f * ((double)z[e] + a.s * acc[e]);
     if (MODE == LK_MEAN || place_ws >= 0) {
         if (!first) return;
         double* r = sr_ws + (MODE == LK_MEAN ? b * a.n_multi + (size_t)a.idx[v] : b * a.n_joins + (size_t)place_ws) * a.D + k.col;
@@ -598,7 +651,7 @@ __global__ __launch_bounds__(kBlock) void lookup_positions_kernel(LkArgs a, cons
     const LkLane k = lk_lane<T>(a.lw, place.tile, a.D);
     if (!place.in || k.valid <= 0) return;
     const LkScal c = scal[b];
-    const double asum = c.ax + c.an, prec1 = c.az + c.lik1;
+    const double asum = c.ax + c.an, f1 = a.s / (c.az + c.lik1);
     const size_t G = kBlock >> a.lw, t0 = (size_t)place.blk * UR * G + k.group;
     int w[UR];
     T v[UR][N], z[UR][N];
@@ -617,7 +670,7 @@ __global__ __launch_bounds__(kBlock) void lookup_positions_kernel(LkArgs a, cons
     for (int i = 0; i < UR; ++i) {
         if (w[i] <= -2) {
 #pragma unroll
-            for (int e = 0; e < N; ++e) sr[i][e] = a.s * (((double)z[i][e] + a.s * (double)v[i][e]) / prec1);
+            for (int e = 0; e < N; ++e) sr[i][e] = f1 * ((double)z[i][e] + a.s * (double)v[i][e]);
         }
         if (t0 + i * G < a.T) lk_position_out<T, ROW>(a, asum, k, b, t0 + i * G, sr[i], v[i], damping, b_old, out, r_out);
     }
@@ -633,7 +686,7 @@ __global__ __launch_bounds__(kBlock) void lookup_positions1_kernel(LkArgs a, con
     const size_t b = place.b, t = ((size_t)place.blk * kBlock + threadIdx.x) * N;
     if (!place.in || t >= a.T) return;
     const LkScal c = scal[b];
-    const double asum = c.ax + c.an, prec1 = c.az + c.lik1;
+    const double asum = c.ax + c.an, f1 = a.s / (c.az + c.lik1);
     const int valid = a.T - t >= N ? N : (int)(a.T - t);
     int w[N];
     T v[N], o[N], old[N];
@@ -654,7 +707,7 @@ __global__ __launch_bounds__(kBlock) void lookup_positions1_kernel(LkArgs a, con
         z[i] = w[i] >= 0 ? sr_ws[b * a.n_multi + (size_t)w[i]] : w[i] == -1 ? 0.0 : (double)bz[b * a.V + (size_t)(-2 - w[i])];
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-        if (w[i] <= -2) z[i] = a.s * ((z[i] + a.s * (double)v[i]) / prec1);
+        if (w[i] <= -2) z[i] = f1 * (z[i] + a.s * (double)v[i]);
         double m = z[i] * asum - (double)v[i];
         if (damping != 0.0) m = damping * (double)old[i] + (1.0 - damping) * m;
         o[i] = T(m);
@@ -707,20 +760,25 @@ extern "C" int tramp_lookup_create(tramp_ctx* ctx, int dtype, size_t n_rows, siz
         const size_t e = dtype_size(dtype), piece = 16 / e, pieces = (n_cols + piece - 1) / piece;
         int lw = 0;
         while (lw < 6 && ((size_t)1 << lw) < pieces) ++lw;
+        // longer rows in tiles of 32 or 16 pieces where tiles of 64 would leave a fifth of the lanes idle and more: 75 pieces in
+        // five tiles of 16 (10^5 positions of 300 f32, gradient 47.8 -> 42.8 us, lookup of 200000 114 -> 96 us).  Not below 64
+        // pieces: 20 pieces as three tiles of 8 gain in one direction and lose in the other (lookup 17 -> 25 us).
+        for (int w = 5; pieces > 64 && w >= 4; --w)
+            if (((((pieces - 1) >> w) + 1) << w) * 5 <= ((((pieces - 1) >> lw) + 1) << lw) * 4) lw = w;
         const size_t tiles = (pieces + ((size_t)1 << lw) - 1) >> lw;
         const int per_wave = kKeep << (6 - lw), per_block = kKeep << (8 - lw);
         const bool short_rows = n_cols * e < 64;
-        std::vector<LkItem> chunks, runs, joins, spreads;
-        std::vector<int> waves, light, single, idx, code;
+        std::vector<LkItem> chunks, runs, joins, spreads, waves, light, single;
+        std::vector<int> idx, code;
         for (size_t v = 0; v < n_rows; ++v) {
             const int c = counts[v], j0 = off[v];
             if (c == 0) continue;
             if (c == 1) {
-                single.push_back((int)v);
+                single.push_back(LkItem{(int)v, j0, j0 + c, perm[(size_t)j0]});
             } else if (c <= kKeep) {
-                light.push_back((int)v);
+                light.push_back(LkItem{(int)v, j0, j0 + c, perm[(size_t)j0]});
             } else if (c <= per_wave) {
-                waves.push_back((int)v);
+                waves.push_back(LkItem{(int)v, j0, j0 + c, -1});
             } else if (c <= per_block) {
                 runs.push_back(LkItem{(int)v, j0, j0 + c, -1});
             } else {
@@ -737,6 +795,8 @@ extern "C" int tramp_lookup_create(tramp_ctx* ctx, int dtype, size_t n_rows, siz
         }
         for (size_t j = seen; j < n_pos; j += (size_t)per_block)
             spreads.push_back(LkItem{-1, (int)j, (int)std::min(n_pos, j + (size_t)per_block), -1});
+        // equal lengths side by side: a wave goes no deeper than its longest run
+        std::stable_sort(light.begin(), light.end(), [](const LkItem& x, const LkItem& y) { return x.end - x.start > y.end - y.start; });
         const size_t n_light2 = light.size();
         light.insert(light.end(), single.begin(), single.end());
         size_t n_multi = 0;
@@ -772,8 +832,8 @@ extern "C" int tramp_lookup_create(tramp_ctx* ctx, int dtype, size_t n_rows, siz
         const size_t o_tok = put(tokens_h, n_pos * 4), o_perm = put(perm.data(), n_pos * 4), o_off = put(off.data(), (n_rows + 1) * 4);
         const size_t o_cnt = put(cval.data(), 2 * K * 8), o_chunks = put(chunks.data(), chunks.size() * sizeof(LkItem));
         const size_t o_joins = put(joins.data(), joins.size() * sizeof(LkItem)), o_spreads = put(spreads.data(), spreads.size() * sizeof(LkItem));
-        const size_t o_runs = put(runs.data(), runs.size() * sizeof(LkItem)), o_waves = put(waves.data(), waves.size() * 4);
-        const size_t o_light = put(light.data(), light.size() * 4), o_idx = put(idx.data(), idx.size() * 4), o_code = put(code.data(), code.size() * 4);
+        const size_t o_runs = put(runs.data(), runs.size() * sizeof(LkItem)), o_waves = put(waves.data(), waves.size() * sizeof(LkItem));
+        const size_t o_light = put(light.data(), light.size() * sizeof(LkItem)), o_idx = put(idx.data(), idx.size() * 4), o_code = put(code.data(), code.size() * 4);
         tramp_lookup* lk = new tramp_lookup();
         *lk = tramp_lookup{};
         (void)hipSetDevice(ctx->device);
@@ -805,8 +865,8 @@ extern "C" int tramp_lookup_create(tramp_ctx* ctx, int dtype, size_t n_rows, siz
         lk->joins = reinterpret_cast<const LkItem*>(m + o_joins);
         lk->spreads = reinterpret_cast<const LkItem*>(m + o_spreads);
         lk->runs = reinterpret_cast<const LkItem*>(m + o_runs);
-        lk->waves = reinterpret_cast<const int*>(m + o_waves);
-        lk->light = reinterpret_cast<const int*>(m + o_light);
+        lk->waves = reinterpret_cast<const LkItem*>(m + o_waves);
+        lk->light = reinterpret_cast<const LkItem*>(m + o_light);
         lk->idx = reinterpret_cast<const int*>(m + o_idx);
         lk->code = reinterpret_cast<const int*>(m + o_code);
         lk->K = (int)K;
@@ -856,9 +916,12 @@ static bool lk_overlap(const void* x, size_t nx, const void* y, size_t ny) {
         default: CALL(LK_LINES);          \
     }
 
-// Instances by XCD (lk_place): worth it while the last round of eight leaves few XCDs idle.
-static int lk_spread(size_t batch, size_t blocks) {
-    return batch > 1 && (batch + 7) / 8 * 8 * 7 <= batch * 8 && (batch + 7) / 8 * 8 * blocks < 0x7fffffffu;
+// Instances by XCD (lk_place): for what is read out of order in elements or rows, while it stays in an L2 of 4 MiB - the table of
+// an instance for a lookup or a message by position (up to twice that: 8 x 20000 x 64 f32 18.2 -> 14.3 us; 64 x 200000 f64 82 ->
+// 53 us), its positions for the sums (64 x 100000 f64, gradient 102 -> 92 us; 8 x 17 MB would be 169 -> 178 us) - and while the
+// last round of eight leaves few XCDs idle.
+static int lk_spread(size_t batch, size_t blocks, size_t bytes, size_t most) {
+    return batch > 1 && bytes <= most && (batch + 7) / 8 * 8 * 7 <= batch * 8 && (batch + 7) / 8 * 8 * blocks < 0x7fffffffu;
 }
 static dim3 lk_grid(size_t batch, size_t blocks, int spread) {
     return spread ? dim3((unsigned)((batch + 7) / 8 * 8 * blocks)) : dim3((unsigned)blocks, (unsigned)batch);
@@ -869,13 +932,13 @@ static int lookup_apply(tramp_ctx* ctx, const tramp_lookup* lk, size_t batch, co
     constexpr size_t N = LkVec<T>::N;
     if (lk->D == 1) {
         const size_t nb = (lk->T + kBlock * N - 1) / (kBlock * N);
-        const int spread = lk_spread(batch, nb);
+        const int spread = lk_spread(batch, nb, lk->V * sizeof(T), 8u << 20);
         hipLaunchKernelGGL((lookup_apply1_kernel<T>), lk_grid(batch, nb, spread), dim3(kBlock), 0, ctx->stream, lk->V, lk->T, lk->s,
                            (unsigned)nb, (unsigned)batch, spread, lk->tok, z, x);
     } else {
         const size_t per = (size_t)4 * (kBlock >> lk->lw), nb = (lk->T + per - 1) / per;
         TRAMP_REQUIRE(ctx, nb * lk->tiles < 0x7fffffffu);
-        const int spread = lk_spread(batch, nb * lk->tiles);
+        const int spread = lk_spread(batch, nb * lk->tiles, lk->V * lk->D * sizeof(T), 8u << 20);
         const dim3 grid = lk_grid(batch, nb * lk->tiles, spread);
 #define LK_CALL(ROW)                                                                                                                   \
     hipLaunchKernelGGL((lookup_apply_kernel<T, ROW>), grid, dim3(kBlock), 0, ctx->stream, lk->V, lk->D, lk->T, lk->s, lk->lw, (unsigned)nb, \
@@ -968,7 +1031,7 @@ static int launch_rows(tramp_ctx* ctx, const tramp_lookup* lk, size_t batch, con
     TRAMP_REQUIRE(ctx, blocks * lk->tiles < 0x7fffffffu && (size_t)lk->n_spreads * lk->tiles < 0x7fffffffu &&
                            (size_t)lk->n_chunks * lk->tiles < 0x7ffffffeu);
     a.blocks = (unsigned)blocks;
-    a.spread = lk_spread(batch, blocks * lk->tiles);
+    a.spread = lk_spread(batch, blocks * lk->tiles, lk->T * lk->D * sizeof(T), 2u << 20);
     // few workgroups and few counts: each makes the scalars for itself, one launch less (V = 1000, 2000 positions 10.2 -> 7.6 us;
     // with up to 4096 workgroups 8 x 60000 x 8 f64 would be 31.5 against 27.1 us)
     const bool self = q && !lk->n_chunks && blocks && blocks * lk->tiles * batch <= 1024 && lk->K <= 4 * kBlock && q->a_new_out != q->az &&
@@ -989,7 +1052,7 @@ static int launch_rows(tramp_ctx* ctx, const tramp_lookup* lk, size_t batch, con
     if (MODE == LK_MEAN) {
         const size_t per = lk->D == 1 ? (size_t)kBlock * LkVec<T>::N : 4 * G, nb = (lk->T + per - 1) / per;
         a.blocks = (unsigned)nb;
-        a.spread = lk_spread(batch, nb * lk->tiles);
+        a.spread = lk_spread(batch, nb * lk->tiles, lk->V * lk->D * sizeof(T), 8u << 20);
         if (lk->D == 1)
             hipLaunchKernelGGL((lookup_positions1_kernel<T>), lk_grid(batch, nb, a.spread), dim3(kBlock), 0, ctx->stream, a, lk->code, w.scal,
                                bz, w.sr, x, damping, b_old, out, r_out);
