@@ -121,6 +121,30 @@ def test_views_at_any_boundary_and_nothing_behind(ctx, dtype):
         assert all(np.array_equal(a, b) for a, b in zip(res, want))
 
 
+@pytest.mark.parametrize("dtype, batch, lengths, inplace", [(np.float64, 6, (1500001, 1000000), False), (np.float64, 6, (1500001, 1000000), True),
+                                                            (np.float32, 1, (30000001, 5, 10000000), True), (np.float32, 37, (300007,), False)])
+def test_large_lists(ctx, dtype, batch, lengths, inplace):
+    "slices of instances, accesses past the caches: the same results, nothing but the arrays touched"
+    import tramp_amd as T
+    rs = np.random.RandomState(4)
+    x = [rs.standard_normal((batch, n)).astype(dtype) * (1 + np.arange(batch)[:, None]) for n in lengths]
+    p = [(0.5 * rs.standard_normal((batch, n))).astype(dtype) for n in lengths]
+    x = [v.astype(dtype) for v in x]
+    g, gp = group(T, ctx, x, dtype), group(T, ctx, p, dtype)
+    out = g if inplace else group(T, ctx, p, dtype)
+    norm, want, c = step_plain(x, p, 1.0)
+    bound = float(np.median(norm)) * 0.9
+    norm, want, c = step_plain(x, p, bound)
+    got = g.limit_step(gp, bound, out=None if inplace else out).get()
+    rel = 2 * (sum(lengths) + 4) * U
+    assert (np.abs(got - norm) <= rel * norm).all()
+    half = np.finfo(dtype).eps / 2
+    for y, w, a, q in zip(get(out), want, x, p):
+        mag = np.abs(q.astype(float)) + np.abs(a.astype(float))
+        assert (np.abs(y - w) <= half * np.abs(w) + (rel + 6 * U) * mag).all()
+    assert all(np.array_equal(a, b) for a, b in zip(get(gp), p))
+
+
 def test_overlaps_are_refused(ctx):
     import tramp_amd as T
     a = ctx.array(np.arange(20.0))

@@ -279,6 +279,80 @@ def test_captured_calls_replay_and_share_workspaces(ctx):
             ctx._call("tramp_graph_destroy", s["graph"])
 
 
+@pytest.mark.parametrize("V, n, D, B, zipf, pad, dtype", [(700001, 600000, 1, 1, None, 0.0, np.float64), (3000, 90000, 7, 1, 1.1, 0.1, np.float64),
+                                                          (500, 80000, 1, 16, 1.0, 0.2, np.float32), (2500, 40001, 3, 16, 1.2, 0.1, np.float32),
+                                                          (20000, 30000, 5, 8, 0.5, 0.0, np.float64), (300, 200000, 33, 3, 1.0, 0.1, np.float32)])
+def test_larger_messages(ctx, V, n, D, B, zipf, pad, dtype):
+    "the forms that only larger calls take: by position, heavy runs, instances by XCD, no token twice; same tolerances"
+    import tramp_amd as T
+    rs = np.random.RandomState(1)
+    tok = rs.permutation(V)[:n] if zipf is None else zipf_tokens(rs, V, n, zipf, pad)
+    ch = T.LookupChannel(tok, V, dim=D, scale=0.7, padding_index=-1, dtype=dtype, ctx=ctx)
+    ref = LookupFactor(tok, V, D, 0.7)
+    z, x = rs.standard_normal((B, V * D)).astype(dtype), rs.standard_normal((B, n * D)).astype(dtype)
+    az, ax = rs.uniform(0.5, 2, B), rs.uniform(0.1, 3, B)
+    args = ctx.scalars(az), ctx.array(z, dtype), ctx.scalars(ax), ctx.array(x, dtype)
+    K = np.unique(ref.count).size
+    k = 2 * (ref.count.max() + 2 * K + 32) * U
+    for direction in ("forward", "backward"):
+        a, b = getattr(ch, f"compute_{direction}_message")(*args)
+        a2, b2 = getattr(ch, f"compute_{direction}_message")(*args)
+        assert np.array_equal(a.get(), a2.get()) and np.array_equal(b.get(), b2.get())       # the same bits every time
+        damped_a, damped_b = ctx.scalars(np.ones(B)), ctx.zeros(b.shape, dtype)
+        getattr(ch, f"compute_{direction}_message")(*args, out_a=damped_a, out_b=damped_b, damping=0.5, old_a=damped_a, old_b=damped_b)
+        r, _ = getattr(ch, f"compute_{direction}_posterior")(*args)
+        A, Bn, R, Db = a.get(), b.get(), r.get(), damped_b.get()
+        for i in {0, B - 1}:
+            ra, rb = getattr(ref, direction)(az[i], z[i], ax[i], x[i])
+            mag = magnitudes(ref, az[i], z[i], ax[i], x[i], ra, direction)
+            assert abs(A[i] - ra) <= 4 * (K + 8) * U * ra
+            assert (np.abs(Bn[i] - rb) <= eps2(dtype) * np.abs(rb) + k * mag).all()
+            assert (np.abs(Db[i] - 0.5 * rb) <= eps2(dtype) * np.abs(0.5 * rb) + k * mag).all()
+            own = z[i] if direction == "backward" else x[i]
+            a_in = az[i] if direction == "backward" else ax[i]
+            # b' = r (a + a') - b on the posterior the same call gives, which is rounded once more
+            lim = k * mag + eps2(dtype) * (np.abs(rb) + np.abs(R[i].astype(float)) * (a_in + ra)) + 4 * U * (np.abs(R[i].astype(float)) * (a_in + ra) + np.abs(own))
+            assert (np.abs(Bn[i] - (R[i].astype(float) * (a_in + ra) - own)) <= lim).all()
+
+
+def test_a_precision_that_is_nan_stays_one(ctx):
+    import tramp_amd as T
+    ch = T.LookupChannel([0, 1, 1], 3, ctx=ctx)
+    for az, ax in ((np.nan, 1.0), (1.0, np.nan)):
+        for m in (ch.compute_forward_message, ch.compute_backward_message):
+            a, _ = m(ctx.scalars(az), ctx.array(np.ones(3)), ctx.scalars(ax), ctx.array(np.ones(3)))
+            assert np.isnan(a.get()).all()
+
+
+def test_offsets_beyond_32_bits(ctx):
+    "2.2e9 components: rows at the far end of x against the definition, the sums against the counts"
+    import tramp_amd as T
+    n, D = 2200000, 1024
+    tok = np.arange(n) % 3
+    tok[-1] = -1
+    ch = T.LookupChannel(tok, 3, dim=D, scale=2.0, padding_index=-1, dtype=np.float32, ctx=ctx)
+    rs = np.random.RandomState(0)
+    z = rs.randint(-8, 9, (3, D)).astype(np.float32)                   # small integers: every sum below is exact
+    zd = ctx.array(z.reshape(1, -1), np.float32)
+    x = ch.lookup(zd)
+    row = lambda buf, t: T.DeviceArray(ctx, (D,), np.float32, ptr=buf.ptr + 4 * t * D, owner=False).get()      # noqa: E731
+    for t in (0, 1, 2**21 - 1, 2**21, 2**21 + 1, n - 3, n - 2):
+        assert np.array_equal(row(x, t), 2 * z[tok[t]])
+    assert np.array_equal(row(x, n - 1), np.zeros(D, np.float32))
+    count = np.bincount(tok[:-1], minlength=3)
+    g = ch.gradient(x).get().reshape(3, D)
+    assert np.array_equal(g, (4.0 * count[:, None] * z.astype(float)).astype(np.float32))
+    a, b = ch.compute_forward_message(ctx.scalars(1.0), zd, ctx.scalars(0.5), x)
+    ref = LookupFactor(tok, 3, 1, 2.0)
+    ra = ref._a(ref.forward_variance(1.0, 0.5), 0.5)
+    prec = 1.0 + 0.5 * 4 * count
+    mean = 2 * (z + 4.0 * count[:, None] * z) / prec[:, None]
+    for t in (0, 2**21, n - 2):
+        want = mean[tok[t]] * (0.5 + ra) - 2 * z[tok[t]]
+        assert np.abs(row(b, t) - want).max() <= 2**-23 * np.abs(want).max() + 1e-9 * np.abs(mean).max() * (0.5 + ra)
+    assert np.array_equal(row(b, n - 1), np.zeros(D, np.float32)) and a.get()[0] == pytest.approx(ra, rel=1e-12)
+
+
 def test_refusals_on_the_device(ctx):
     import tramp_amd as T
     ch = T.LookupChannel([0, 1, 1], 2, ctx=ctx)

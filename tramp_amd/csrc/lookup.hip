@@ -83,7 +83,8 @@ __device__ __forceinline__ LkScal lk_scalars(const LkScalArgs& q, size_t b, bool
     const int K = q.K, dir = q.dir;
     const double* cnt = q.cnt;
     const double s = q.s;
-    const double ax = q.ax[b], az = dir == TRAMP_BWD ? fmax(1e-11, q.az[b]) : q.az[b];     // linear_channel.py:92-94
+    const double ax = q.ax[b], az_in = q.az[b];
+    const double az = dir == TRAMP_BWD && az_in < 1e-11 ? 1e-11 : az_in;       // linear_channel.py:92-94 (a NaN stays one)
     const double lik1 = ax * s * s;
     double sv = 0.0, sn = 0.0, se = 0.0;
     for (int k = threadIdx.x; k < K; k += kBlock) {
@@ -126,9 +127,9 @@ __device__ __forceinline__ LkScal lk_scalars(const LkScalArgs& q, size_t b, bool
 __global__ __launch_bounds__(kBlock) void lookup_scalars_kernel(LkScalArgs q) { (void)lk_scalars(q, blockIdx.x, true); }
 
 // ---------------------------------------------------------------- rows in 16-byte pieces
-// A row of D elements is walked by LPR = min(64, 2^ceil(log2(D / N))) lanes, one 16-byte piece (N elements) per lane, in
-// column tiles of LPR pieces where the row is longer (1 KiB per wave and row).  The pieces start wherever the row does: a
-// 16-byte access needs element alignment only, so odd D and views cost nothing but the last piece of a row (TAIL).
+// A row of D elements is walked by LPR lanes, one 16-byte piece (N elements) per lane: the power of two that holds the row, up to
+// 64, and column tiles of LPR pieces where the row is longer (tramp_lookup_create).  The pieces start wherever the row does: a
+// 16-byte access needs element alignment only, so odd D and views cost nothing but the last piece of a row (LK_TAIL).
 template <typename T> struct LkVec;
 template <> struct LkVec<float> {
     typedef float U __attribute__((ext_vector_type(4), aligned(4)));
@@ -219,10 +220,13 @@ __device__ __forceinline__ LkPlace lk_place(unsigned blocks, unsigned tiles, uns
 }
 
 // ---------------------------------------------------------------- x = scale z[token]
-// Bound by the write of x (and the read of the distinct rows of z).  Four rows per group in flight.
+// Bound by the write of x (and the read of the distinct rows of z).  Four rows per group in flight.  65536 positions of 1024 f32
+// from 32000 rows, 316 MB: 46 us, 6.8 TB/s (a copy of that size from memory runs at 5.2; most of z comes from the cache, which
+// the non-temporal stores of x leave alone: 80 us with ordinary ones).
 template <typename T, int ROW>
 __global__ __launch_bounds__(kBlock) void lookup_apply_kernel(size_t V, size_t D, size_t n_pos, double s, int lw, unsigned blocks,
-                                                              unsigned tiles, unsigned batch, int spread, const int* __restrict__ tok, const T* __restrict__ z, T* __restrict__ x) {
+                                                              unsigned tiles, unsigned batch, int spread, const int* __restrict__ tok,
+                                                              const T* __restrict__ z, T* __restrict__ x) {
     constexpr int N = LkVec<T>::N, UR = 4;
     const LkPlace w = lk_place(blocks, tiles, batch, spread);
     const size_t b = w.b;
@@ -253,8 +257,7 @@ __global__ __launch_bounds__(kBlock) void lookup_apply_kernel(size_t V, size_t D
 // one column: N positions per lane, written as one piece
 template <typename T>
 __global__ __launch_bounds__(kBlock) void lookup_apply1_kernel(size_t V, size_t n_pos, double s, unsigned blocks, unsigned batch, int spread,
-                                                               const int* __restrict__ tok,
-                                                               const T* __restrict__ z, T* __restrict__ x) {
+                                                               const int* __restrict__ tok, const T* __restrict__ z, T* __restrict__ x) {
     constexpr int N = LkVec<T>::N;
     const LkPlace w = lk_place(blocks, 1, batch, spread);
     const size_t b = w.b, t = ((size_t)w.blk * kBlock + threadIdx.x) * N;
@@ -281,7 +284,6 @@ __global__ __launch_bounds__(kBlock) void lookup_apply1_kernel(size_t V, size_t 
 // kKeep: 8 rows in flight per group leave 5 to 8 waves per SIMD; 16 leave 3 to 5 and cost a third (gradient 121 against 84 us,
 // message to 10^6 positions of 64 columns 136 against 104 us), 4 make longer runs of every kind (89 and 103 us).
 constexpr int kKeep = 8;
-
 
 struct LkArgs {
     const int* off;
@@ -823,6 +825,8 @@ extern "C" int tramp_lookup_create(tramp_ctx* ctx, int dtype, size_t n_rows, siz
         cval.insert(cval.end(), cmul.begin(), cmul.end());
         // one allocation: the arrays one behind the other
         std::vector<char> host;
+        host.reserve(n_pos * (short_rows ? 12 : 8) + n_rows * (short_rows ? 8 : 4) + 2 * K * 8 + 16 * 256 +
+                     sizeof(LkItem) * (chunks.size() + joins.size() + spreads.size() + runs.size() + waves.size() + light.size()));
         auto put = [&host](const void* p, size_t bytes) {
             const size_t at = host.size();
             host.resize(at + ((bytes + 255) & ~(size_t)255));
