@@ -54,6 +54,33 @@ def test_valid_arguments_reach_the_library():
         T.get_channel("lookup", tokens=np.uint8([0, 1]), n_tokens=2, ctx=HostContext())
 
 
+@pytest.mark.parametrize("dtype", [np.uint8, np.uint16, np.uint32, np.uint64, np.int8, np.int16, np.int64])
+def test_padded_positions_of_any_integer_type(dtype):
+    "-1 where padded, also where the type cannot hold it and the table is longer than its largest value"
+    seen = []
+
+    class Recorder(HostContext):
+        def _call(self, name, dt, rows, cols, n, tokens, *rest):
+            seen.extend((C.c_int * n).from_address(tokens))
+            raise AssertionError(name)
+
+    last = int(np.iinfo(dtype).max)
+    with pytest.raises(AssertionError, match="tramp_lookup_create"):
+        T.LookupChannel(np.array([0, last, 5, 1], dtype=dtype), 70000, padding_index=last, ctx=Recorder())
+    assert seen == [0, -1, 5, 1]
+
+
+def test_the_largest_sizes_are_refused_before_anything_is_allocated():
+    many = np.broadcast_to(np.int8(0), (2**31 - 2**16 + 1,))             # one byte of memory
+    with pytest.raises(ValueError, match="exceed"):
+        T.LookupChannel(many, 3, ctx=HostContext())
+    for kw in (dict(n_tokens=2**31 - 2**16 + 1), dict(n_tokens=3, dim=2**31 - 2**16 + 1)):
+        with pytest.raises(ValueError, match="exceed"):
+            T.LookupChannel([0], ctx=HostContext(), **kw)
+    with pytest.raises(AssertionError, match="tramp_lookup_create"):
+        T.LookupChannel([0], 2**31 - 2**16, ctx=HostContext())
+
+
 def test_array_group_refuses():
     ctx, other = HostContext(), HostContext()
     a = fake(ctx, (2, 5))

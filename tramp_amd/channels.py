@@ -1503,8 +1503,8 @@ class LookupChannel(Channel):
         if tok.size < 1:
             raise ValueError("tokens is empty")
         cols = self.dim or 1
-        if max(tok.size, self.n_tokens, cols) >= 2**31 - 1:
-            raise ValueError("positions, rows and columns must stay below 2^31 - 1")
+        if max(tok.size, self.n_tokens, cols) > 2**31 - 2**16:
+            raise ValueError("positions, rows and columns must not exceed 2^31 - 2^16")
         scale = float(scale)
         if not np.isfinite(scale) or scale == 0.0:
             raise ValueError(f"scale must be finite and not zero, got {scale}")
@@ -1519,7 +1519,8 @@ class LookupChannel(Channel):
         self._xshape = tok.shape + (() if self.dim is None else (self.dim,)) or (1,)
         self.Nz, self.Nx = self.n_tokens * cols, tok.size * cols
         self.alpha = self.Nx / self.Nz
-        host = np.ascontiguousarray(np.where(padded, -1, tok).reshape(-1), dtype=np.int32)
+        host = tok.reshape(-1).astype(np.int32)            # the rows read fit; what a padded position held is replaced
+        host[padded.reshape(-1)] = -1
         self._seen = int(read.size)
         self._tokens_h = host
         h = C.c_void_p()

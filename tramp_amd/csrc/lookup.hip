@@ -740,7 +740,8 @@ extern "C" int tramp_lookup_create(tramp_ctx* ctx, int dtype, size_t n_rows, siz
     *out = nullptr;
     TRAMP_REQUIRE(ctx, dtype == TRAMP_F32 || dtype == TRAMP_F64);
     TRAMP_REQUIRE(ctx, n_rows > 0 && n_cols > 0 && n_pos > 0 && tokens_h);
-    TRAMP_REQUIRE(ctx, n_rows < 0x7fffffffu && n_cols < 0x7fffffffu && n_pos < 0x7fffffffu);
+    constexpr size_t most = 0x7fff0000u;                           // the strided loops step beyond the last position in 32 bits
+    TRAMP_REQUIRE(ctx, n_rows <= most && n_cols <= most && n_pos <= most);
     TRAMP_REQUIRE(ctx, scale - scale == 0.0);
     TRAMP_REQUIRE(ctx, !ctx->capturing);
     for (size_t t = 0; t < n_pos; ++t)
