@@ -174,6 +174,40 @@ def test_overlaps_are_refused(ctx):
     assert np.array_equal(a.get(), np.arange(20.0))
 
 
+def test_norms_and_precisions_inside_a_list_are_refused(ctx):
+    import tramp_amd as T
+    E = T._lib.TrampHipError
+    m = ctx.array(np.arange(40.0))
+    view = lambda lo, *shape: T.DeviceArray(ctx, shape, np.float64, ptr=m.ptr + 8 * lo, owner=False)      # noqa: E731
+    g, prev, out = (T.ArrayGroup([view(lo, 2, 2), view(lo + 4, 2, 3)]) for lo in (0, 10, 20))
+    apart = T.ArrayGroup([view(0, 2, 2)])
+    a, a_prev, norm = view(30, 1, 2), view(32, 1, 2), view(34, 2)
+    for bad in (view(9, 2), view(0, 2), view(3, 2)):
+        with pytest.raises(E):
+            g.norm(bad)
+        with pytest.raises(E):
+            g.clip(1.0, norm=bad)
+    with pytest.raises(E):
+        g.clip(1.0, out=out, norm=view(28, 2))
+    for kw in (dict(norm=view(9, 2)), dict(norm=view(10, 2)), dict(norm=view(29, 2)), dict(norm=view(31, 2)), dict(norm=view(33, 2)),
+               dict(a=view(0, 1, 2)), dict(a=view(29, 1, 2)), dict(a_prev=view(18, 1, 2)), dict(a_prev=view(31, 1, 2))):
+        with pytest.raises(E):
+            g.limit_step(prev, 1.0, out=out, **dict(dict(norm=norm, a=a, a_prev=a_prev), **kw))
+    apart.norm(view(4, 2))                                             # right behind the array
+    assert np.array_equal(m.get()[np.r_[:4, 6:40]], np.arange(40.0)[np.r_[:4, 6:40]])
+    g.limit_step(prev, 1.0, out=out, norm=norm, a=a, a_prev=a_prev)
+
+
+def test_precisions_that_are_infinite_stay_so(ctx):
+    import tramp_amd as T
+    for n in (3, 50000):                                               # one launch, two launches
+        x, p = T.ArrayGroup([ctx.array(np.full((1, n), 2.0))]), T.ArrayGroup([ctx.zeros((1, n), np.float64)])
+        a, a_prev = ctx.array(np.array([[np.inf], [4.0], [np.inf]])), ctx.array(np.array([[np.inf], [2.0], [1.0]]))
+        norm = x.limit_step(p, np.sqrt(n), a=a, a_prev=a_prev).get()   # factor 1/2
+        assert norm[0] == pytest.approx(2 * np.sqrt(n), rel=1e-14)
+        assert a.get()[:, 0] == pytest.approx([np.inf, 3.0, np.inf], rel=1e-14)
+
+
 def test_replays_equal_the_eager_calls(ctx):
     import tramp_amd as T
     rs = np.random.RandomState(9)

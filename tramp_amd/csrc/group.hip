@@ -186,7 +186,7 @@ template <bool STEP> __device__ __forceinline__ void group_side(const GroupSide&
     if (!STEP) return;
     for (size_t i = threadIdx.x; i < q.n_a; i += kBlock) {
         const double o = q.a_prev[i * q.batch + b], x = q.a[i * q.batch + b];
-        const double r = c < 1.0 ? o + c * (x - o) : x;
+        const double r = c < 1.0 && x != o ? o + c * (x - o) : x;          // infinite before and after: so it stays
         q.a[i * q.batch + b] = r;
         if (q.refresh) q.a_prev[i * q.batch + b] = r;
     }
@@ -332,6 +332,14 @@ static int check_pair(tramp_ctx* ctx, const tramp_group* g, const tramp_group* o
     return TRAMP_OK;
 }
 
+// n doubles of the caller's (norms, precisions) that touch no array of g
+static bool clear_of(const tramp_group* g, const double* p, size_t n) {
+    const uintptr_t lo = (uintptr_t)p, hi = lo + n * sizeof(double);
+    const tramp_group::Span* it = std::lower_bound(g->span, g->span + g->n_span, hi, [](const tramp_group::Span& s, uintptr_t x) { return s.lo < x; });
+    return !p || it == g->span || (it - 1)->hi <= lo;
+}
+static bool apart(const double* p, size_t n, const double* q, size_t m) { return !p || !q || p + n <= q || q + m <= p; }
+
 // workgroups per instance: about kBlocks in all, each with the same number of chunks
 static int partials_of(const tramp_group* g, size_t batch) {
     if (g->nchunk < 1) return 1;
@@ -379,6 +387,7 @@ static int group_run(tramp_ctx* ctx, const tramp_group* g, const tramp_group* pr
 extern "C" int tramp_group_norm(tramp_ctx* ctx, const tramp_group* g, double* norm_d) {
     if (!ctx) return TRAMP_EINVAL;
     TRAMP_REQUIRE(ctx, g && norm_d && g->device == ctx->device);
+    TRAMP_REQUIRE(ctx, clear_of(g, norm_d, g->batch));
     const GroupSide q{0.0, norm_d, nullptr, nullptr, 0, g->batch, 0};
     return g->dtype == TRAMP_F64 ? group_run<double, false>(ctx, g, nullptr, nullptr, q)
                                  : group_run<float, false>(ctx, g, nullptr, nullptr, q);
@@ -390,6 +399,7 @@ extern "C" int tramp_group_clip(tramp_ctx* ctx, const tramp_group* g, double max
     TRAMP_REQUIRE(ctx, max_norm > 0.0);
     int rc = check_pair(ctx, g, out, true, "tramp_group_clip");
     if (rc) return rc;
+    TRAMP_REQUIRE(ctx, clear_of(g, norm_d, g->batch) && clear_of(out, norm_d, g->batch));
     const GroupSide q{max_norm, norm_d, nullptr, nullptr, 0, g->batch, 0};
     return g->dtype == TRAMP_F64 ? group_run<double, false>(ctx, g, nullptr, out, q)
                                  : group_run<float, false>(ctx, g, nullptr, out, q);
@@ -401,7 +411,11 @@ extern "C" int tramp_group_limit_step(tramp_ctx* ctx, const tramp_group* g, cons
     TRAMP_REQUIRE(ctx, g && prev && out && g->device == ctx->device);
     TRAMP_REQUIRE(ctx, max_step > 0.0);
     TRAMP_REQUIRE(ctx, n_a == 0 || (a_d && a_prev_d));
-    TRAMP_REQUIRE(ctx, n_a == 0 || a_d + n_a * g->batch <= a_prev_d || a_prev_d + n_a * g->batch <= a_d);
+    const size_t na = n_a * g->batch;
+    if (!n_a) a_d = a_prev_d = nullptr;
+    TRAMP_REQUIRE(ctx, apart(a_d, na, a_prev_d, na) && apart(a_d, na, norm_d, g->batch) && apart(a_prev_d, na, norm_d, g->batch));
+    for (const tramp_group* l : {g, prev, out})
+        TRAMP_REQUIRE(ctx, clear_of(l, norm_d, g->batch) && clear_of(l, a_d, na) && clear_of(l, a_prev_d, na));
     int rc = check_pair(ctx, g, prev, false, "tramp_group_limit_step");
     if (!rc) rc = check_pair(ctx, g, out, true, "tramp_group_limit_step");
     if (!rc) rc = check_pair(ctx, prev, out, false, "tramp_group_limit_step");
