@@ -314,6 +314,42 @@ def test_bounded_sweeps_match_the_plain_loop(ctx, kind, damping, max_step):
             assert np.array_equal(other.get_variables_data()[name]["r"], r[name]["r"]), name
 
 
+def conv_problem(T, ctx, depth):
+    "a convolution (depth 1), or a dense layer and a convolution (depth 2): channels that keep projections of messages"
+    rs = np.random.RandomState(21)
+    n, B = 64, 2
+    filt = rs.standard_normal(n) / 8
+    W = np.stack([np.roll(filt, i) for i in range(n)])                    # x_i = sum_j f[j - i] z_j, roll(f, i)[j] = f[j - i]
+    W0 = orc.gaussian_ensemble(rs, n, 40)
+    Y = rs.standard_normal((B, n))
+    conv, z = T.ConvChannel(filt, ctx=ctx), T.SISOVariable(id="z")
+    assert np.abs(conv.sample(np.eye(n)).T - W).max() < 1e-13
+    end = conv @ T.SISOVariable(id="c") @ T.GaussianLikelihood(y=Y, var=0.3, ctx=ctx)
+    fac = lambda b: [orc.LinearFactor(W), orc.GaussLikFactor(Y[b], 0.3)]               # noqa: E731
+    if depth == 1:
+        model = T.GaussBernoulliPrior(size=n, rho=0.5, ctx=ctx) @ z @ end
+        return model.to_model(), lambda b: [orc.GBPriorFactor(n, rho=0.5)] + fac(b), [n, n], ("z", "c")
+    model = (T.GaussBernoulliPrior(size=40, rho=0.5, ctx=ctx) @ T.SISOVariable(id="x") @ T.LinearChannel(W0, ctx=ctx, svd="host") @ z @ end)
+    return model.to_model(), lambda b: [orc.GBPriorFactor(40, rho=0.5), orc.LinearFactor(W0)] + fac(b), [40, n, n], ("x", "z", "c")
+
+
+@pytest.mark.parametrize("graph", [False, True])
+@pytest.mark.parametrize("restore", [False, True])
+@pytest.mark.parametrize("depth", [1, 2])
+def test_bounded_sweeps_over_channels_that_cache_projections(ctx, depth, restore, graph):
+    import tramp_amd as T
+    model, factors, sizes, names = conv_problem(T, ctx, depth)
+    ep = T.ExpectationPropagation(model, ctx=ctx)
+    ep.iterate(max_iter=9, callback=T.EarlyStoppingEP(tol=0.0, max_increase=np.inf), damping=0.1, max_step=4.0, restore_messages=restore, graph=graph)
+    r, norms = ep.get_variables_data(), ep.step_norm.get()
+    for b in range(2):
+        want, nn = ep_plain(factors(b), sizes, 4.0, 0.1, 9)
+        assert nn[0] > 4.0                                             # the bound is at work
+        for i, name in enumerate(names):
+            assert np.abs(r[name]["r"][b] - want[i]).max() < 1e-8 * np.abs(want[i]).max(), (name, b)
+        assert norms[b] == pytest.approx(nn[-1], rel=1e-6)
+
+
 def test_a_wide_bound_changes_nothing_and_bounds_end_with_their_call(ctx):
     import tramp_amd as T
     make, _, _, _ = problem(T, ctx, "lookup")

@@ -433,6 +433,41 @@ def test_ep_matches_the_dense_channel_and_the_oracle(ctx, damping, graph):
     np.testing.assert_allclose(ep.log_evidence(), dense.log_evidence(), rtol=1e-8)
 
 
+def test_adaptive_damping_matches_the_dense_channel(ctx):
+    "the step-halving search evaluates messages and log-partitions of candidates: the same trajectory as the one-hot matrix"
+    import tramp_amd as T
+    rs = np.random.RandomState(8)
+    V, n = 40, 90
+    tok = zipf_tokens(rs, V, n, 0.7, 0.1)
+    W = dense_of(tok, V, 1, 1.2)
+    y = W @ orc.gb_sample(rs, V, 0.5) + np.sqrt(0.1) * rs.standard_normal(n)
+    r, logz = [], []
+    for ch in (T.LookupChannel(tok, V, scale=1.2, padding_index=-1, ctx=ctx), T.LinearChannel(W, ctx=ctx, svd="host")):
+        ep = T.ExpectationPropagation(regression(T, ctx, ch, V, y), ctx=ctx)
+        ep.iterate(max_iter=6, callback=T.PassCallback(), damping="adaptive")
+        r.append(ep.get_variables_data()["x"]["r"].reshape(-1))
+        logz.append(ep.log_evidence())
+    assert np.abs(r[0] - r[1]).max() < 1e-7 * np.abs(r[1]).max()
+    assert logz[0] == pytest.approx(logz[1], rel=1e-7)
+
+
+def test_one_table_read_twice_in_a_tree(ctx):
+    "x feeds two lookups with tokens of their own: the exact posterior of the Gaussian model"
+    import tramp_amd as T
+    rs = np.random.RandomState(10)
+    V, n1, n2 = 20, 70, 33
+    t1, t2 = rs.randint(0, V, n1), zipf_tokens(rs, V, n2, 1.0, 0.2)
+    y1, y2 = rs.standard_normal(n1), rs.standard_normal(n2)
+    W1, W2 = dense_of(t1, V, 1, 1.0), dense_of(t2, V, 1, 0.5)
+    want = np.linalg.solve(np.eye(V) + W1.T @ W1 / 0.2 + W2.T @ W2 / 0.4, W1.T @ y1 / 0.2 + W2.T @ y2 / 0.4)
+    model = (T.GaussianPrior(size=V, ctx=ctx) @ T.SIMOVariable(id="x", n_next=2) @ (
+        (T.LookupChannel(t1, V, ctx=ctx) @ T.SISOVariable(id="z1") @ T.GaussianLikelihood(y=y1, var=0.2, ctx=ctx))
+        + (T.LookupChannel(t2, V, scale=0.5, padding_index=-1, ctx=ctx) @ T.SISOVariable(id="z2") @ T.GaussianLikelihood(y=y2, var=0.4, ctx=ctx)))).to_model()
+    ep = T.ExpectationPropagation(model, ctx=ctx)
+    ep.iterate(max_iter=500, damping=0.3, callback=T.EarlyStoppingEP(tol=1e-10, max_increase=np.inf))
+    assert np.abs(ep.get_variables_data()["x"]["r"].reshape(-1) - want).max() < 1e-6
+
+
 def test_state_evolution_sampling_and_tables(ctx):
     "a table of D columns, positions of two axes; SE against the dense channel of the same matrix"
     import tramp_amd as T
