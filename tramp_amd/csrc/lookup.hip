@@ -296,6 +296,7 @@ struct LkArgs {
     const int* idx;
     size_t V, D, T;
     unsigned n_chunks, n_joins, n_runs, n_waves, wave_blocks, n_light, n_multi, blocks, tiles, batch;
+    unsigned n_lead;             // chunks summed in the launch of the runs (gradient)
     int lw, spread;
     double s;
 };
@@ -410,25 +411,18 @@ __device__ __forceinline__ void lk_position_out(const LkArgs& a, double asum, co
     }
 }
 
-// First launch: the partial sums of the heavy runs; one more workgroup per instance makes its scalars.
+// the partial sum of a chunk of a heavy run
 template <typename T, int ROW, bool ONCE>
-__global__ __launch_bounds__(kBlock) void lookup_chunks_kernel(LkArgs a, LkScalArgs q, const T* __restrict__ x, double* __restrict__ partials) {
+__device__ __forceinline__ void lk_chunk(const LkArgs& a, const LkLane& k, size_t b, unsigned blk, const T* __restrict__ xb,
+                                         double* __restrict__ partials, double (*sm)[kWave][LkVec<T>::N]) {
     constexpr int N = LkVec<T>::N;
-    __shared__ double sm[kBlock / kWave][kWave][N];
-    const size_t b = blockIdx.y;
-    if (blockIdx.x == a.n_chunks * a.tiles) {
-        (void)lk_scalars(q, b, true);
-        return;
-    }
-    const unsigned blk = blockIdx.x / a.tiles;
-    const LkLane k = lk_lane<T>(a.lw, blockIdx.x - blk * a.tiles, a.D);
     const LkItem it = a.chunks[blk];
     double acc[N];
     int pj[kKeep];
     T rows[kKeep][N];
 #pragma unroll
     for (int e = 0; e < N; ++e) acc[e] = 0.0;
-    if (k.valid > 0) lk_gather<T, ROW, kKeep, false, ONCE>(a, x + b * a.T * a.D, k, it.start, it.end - it.start, k.group, 8 - a.lw, -1, acc, pj, rows);
+    if (k.valid > 0) lk_gather<T, ROW, kKeep, false, ONCE>(a, xb, k, it.start, it.end - it.start, k.group, 8 - a.lw, -1, acc, pj, rows);
     lk_block_join<N>(k, acc, sm);
     if (threadIdx.x >= (1u << a.lw) || k.valid <= 0) return;
     double* p = partials + (b * a.n_chunks + (size_t)it.slot) * a.D + k.col;
@@ -437,11 +431,26 @@ __global__ __launch_bounds__(kBlock) void lookup_chunks_kernel(LkArgs a, LkScalA
         if (e < k.valid) p[e] = acc[e];
 }
 
-// Second launch: every run.  Workgroups, in this order: joins of the partial sums, block runs, wave runs, light ones.
+// First launch: the partial sums of the heavy runs; one more workgroup per instance makes its scalars.
+template <typename T, int ROW, bool ONCE>
+__global__ __launch_bounds__(kBlock) void lookup_chunks_kernel(LkArgs a, LkScalArgs q, const T* __restrict__ x, double* __restrict__ partials) {
+    __shared__ double sm[kBlock / kWave][kWave][LkVec<T>::N];
+    const size_t b = blockIdx.y;
+    if (blockIdx.x == a.n_chunks * a.tiles) {
+        (void)lk_scalars(q, b, true);
+        return;
+    }
+    const unsigned blk = blockIdx.x / a.tiles;
+    const LkLane k = lk_lane<T>(a.lw, blockIdx.x - blk * a.tiles, a.D);
+    lk_chunk<T, ROW, ONCE>(a, k, b, blk, x + b * a.T * a.D, partials, sm);
+}
+
+// Second launch: every run.  Workgroups, in this order: joins of the partial sums, block runs, wave runs, light ones.  The gradient
+// needs no scalars: with short rows its chunks lead this launch and only their joins are left for another.
 template <typename T, int ROW, int MODE, bool SELF>
 __global__ __launch_bounds__(kBlock) void lookup_rows_kernel(LkArgs a, LkScalArgs q, const LkScal* __restrict__ scal, const T* __restrict__ bz,
                                                              const T* __restrict__ x, double damping, const T* b_old, T* out,
-                                                             T* __restrict__ r_out, const double* __restrict__ partials,
+                                                             T* __restrict__ r_out, double* __restrict__ partials,
                                                              double* __restrict__ sr_ws) {
     constexpr int N = LkVec<T>::N;
     __shared__ double sm[kBlock / kWave][kWave][N];
@@ -453,6 +462,13 @@ __global__ __launch_bounds__(kBlock) void lookup_rows_kernel(LkArgs a, LkScalArg
     LkScal c{};
     if (MODE != LK_GRAD) c = SELF ? lk_scalars(q, b, place.blk == 0 && place.tile == 0) : scal[b];
     const T* xb = x + b * a.T * a.D;
+    if (MODE == LK_GRAD && ROW != LK_LINES) {                      // lines are no short rows
+        if (blk < a.n_lead) {
+            lk_chunk<T, ROW, true>(a, k, b, blk, xb, partials, sm);
+            return;
+        }
+        blk -= a.n_lead;
+    }
     const bool act = k.valid > 0;
     double acc[N];
     int pj[kKeep];
@@ -1032,7 +1048,11 @@ static int launch_rows(tramp_ctx* ctx, const tramp_lookup* lk, size_t batch, con
     a.lw = lk->lw;
     a.s = lk->s;
     const size_t G = kBlock >> lk->lw;
-    const size_t blocks = (size_t)a.n_joins + a.n_runs + a.wave_blocks + ((size_t)a.n_light + G - 1) / G;
+    // short rows: 64 x 60000 f32 of one column 27.2 -> 21.5 us, 1000001 f64 21.9 -> 20.1, 8 x 200000 x 7 f64 43.4 -> 41.2; longer ones
+    // would lose: 65536 x 1024 f32 78.7 against 83.1 us, 20000 x 300 f64 15.2 against 16.1
+    a.n_lead = MODE == LK_GRAD && lk->short_rows ? lk->n_chunks : 0;
+    if (a.n_lead) a.n_joins = 0;
+    const size_t blocks = (size_t)a.n_lead + a.n_joins + a.n_runs + a.wave_blocks + ((size_t)a.n_light + G - 1) / G;
     TRAMP_REQUIRE(ctx, blocks * lk->tiles < 0x7fffffffu && (size_t)lk->n_spreads * lk->tiles < 0x7fffffffu &&
                            (size_t)lk->n_chunks * lk->tiles < 0x7ffffffeu);
     a.blocks = (unsigned)blocks;
@@ -1041,7 +1061,7 @@ static int launch_rows(tramp_ctx* ctx, const tramp_lookup* lk, size_t batch, con
     // with up to 4096 workgroups 8 x 60000 x 8 f64 would be 31.5 against 27.1 us)
     const bool self = q && !lk->n_chunks && blocks && blocks * lk->tiles * batch <= 1024 && lk->K <= 4 * kBlock && q->a_new_out != q->az &&
                       q->a_new_out != q->ax;
-    if (lk->n_chunks || (q && !self))
+    if ((lk->n_chunks && !a.n_lead) || (q && !self))
         hipLaunchKernelGGL((lookup_chunks_kernel<T, ROW, MODE != LK_FWD && MODE != LK_MEAN>), dim3(lk->n_chunks * lk->tiles + (q ? 1 : 0), (unsigned)batch),
                            dim3(kBlock), 0, ctx->stream, a, q ? *q : LkScalArgs{}, x, w.partials);
     const dim3 grid = lk_grid(batch, blocks * lk->tiles, a.spread);
@@ -1051,6 +1071,14 @@ static int launch_rows(tramp_ctx* ctx, const tramp_lookup* lk, size_t batch, con
     else if (blocks)
         hipLaunchKernelGGL((lookup_rows_kernel<T, ROW, MODE, false>), grid, dim3(kBlock), 0, ctx->stream, a, LkScalArgs{}, w.scal, bz, x, damping,
                            b_old, out, r_out, w.partials, w.sr);
+    if (a.n_lead) {
+        LkArgs j = a;
+        j.n_joins = j.blocks = lk->n_joins;
+        j.n_lead = j.n_runs = j.n_waves = j.wave_blocks = j.n_light = 0;
+        j.spread = 0;
+        hipLaunchKernelGGL((lookup_rows_kernel<T, ROW, MODE, false>), lk_grid(batch, (size_t)j.blocks * lk->tiles, 0), dim3(kBlock), 0, ctx->stream,
+                           j, LkScalArgs{}, w.scal, bz, x, damping, b_old, out, r_out, w.partials, w.sr);
+    }
     if (MODE == LK_FWD && lk->n_spreads)
         hipLaunchKernelGGL((lookup_spread_kernel<T, ROW>), dim3(lk->n_spreads * lk->tiles, (unsigned)batch), dim3(kBlock), 0, ctx->stream, a,
                            lk->spreads, w.scal, w.sr, x, damping, b_old, out, r_out);
