@@ -576,7 +576,7 @@ int tramp_lookup_gradient(tramp_ctx* ctx, tramp_lookup* lookup, size_t batch, co
 int tramp_lookup_variance(tramp_ctx* ctx, tramp_lookup* lookup, int dir, size_t batch, const double* az_d, const double* ax_d,
                           double* v_d, double* a_new_d, double* n_eff_d);
 /* dir BWD: the message to z ([batch, n_rows, n_cols]), FWD: to x ([batch, n_pos, n_cols]); r_d, v_d optional posterior.
- * b_new_d and r_d must not overlap bz_d, bx_d or each other; a_old_d / b_old_d may be the outputs. */
+ * b_new_d and r_d must not overlap bz_d, bx_d or each other, nor r_d b_old_d; a_old_d / b_old_d may be a_new_d / b_new_d. */
 int tramp_lookup_message(tramp_ctx* ctx, tramp_lookup* lookup, int dir, size_t batch, const double* az_d, const void* bz_d,
                          const double* ax_d, const void* bx_d, double damping, const double* a_old_d, const void* b_old_d,
                          double* a_new_d, void* b_new_d, void* r_d, double* v_d);

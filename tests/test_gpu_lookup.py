@@ -388,6 +388,10 @@ def test_refusals_on_the_device(ctx):
     assert np.array_equal(big.get(), np.zeros(12))
     with pytest.raises(T._lib.TrampHipError):
         ctx._call("tramp_lookup_message", ch._handle, 0, 1, a.ptr, z.ptr, a.ptr, x.ptr, 0.5, None, None, a.ptr, ctx.empty(3).ptr, None, None)
+    old = ctx.zeros((1, 3))                                            # the posterior over the old message
+    with pytest.raises(T._lib.TrampHipError):
+        ctx._call("tramp_lookup_message", ch._handle, T._lib.FWD, 1, a.ptr, z.ptr, a.ptr, x.ptr, 0.5, a.ptr, old.ptr, a.ptr,
+                  ctx.empty((1, 3)).ptr, old.ptr, None)
     h = C.c_void_p()
     bad = np.array([0, 5], dtype=np.int32)
     for args in ((1, 2, 1, 2, bad.ctypes.data, 1.0), (1, 2, 0, 2, bad.ctypes.data, 1.0), (7, 9, 1, 2, bad.ctypes.data, 1.0),

@@ -192,7 +192,9 @@ template <bool STEP> __device__ __forceinline__ void group_side(const GroupSide&
     }
 }
 
-// The two passes.  Rows y of the grid: the instances [a0, a0 + n_apply), whose sums an earlier launch has left, are finished;
+// The two passes.  Bound by memory: x (and prev) twice, the second time from the cache as far as it reaches, out once.
+// 10^9 bytes of f32 in 24 arrays clipped in place 495 us (2 GB at a copy's 5.14 TB/s: 389 us), 64 instances of 300000 f64 with their
+// previous values 130 us (461 MB: 90 us), 20 MB in 41 arrays 15 us (7.8 us).  Rows y of the grid: the instances [a0, a0 + n_apply), whose sums an earlier launch has left, are finished;
 // of the following ones the sums are taken.
 template <typename T, bool STEP, bool ONCE>
 __global__ __launch_bounds__(kBlock) void group_pass_kernel(unsigned nchunk, const GroupChunk* __restrict__ xs, const GroupChunk* __restrict__ ps,
@@ -215,7 +217,7 @@ __global__ __launch_bounds__(kBlock) void group_pass_kernel(unsigned nchunk, con
     }
 }
 
-// small instances: one workgroup each does both passes in one launch
+// small instances: one workgroup each does both passes in one launch; bound by its latency (4 arrays, 3000 f64 in all: 6.2 us)
 template <typename T, bool STEP>
 __global__ __launch_bounds__(kBlock) void group_small_kernel(unsigned nchunk, const GroupChunk* __restrict__ xs, const GroupChunk* __restrict__ ps,
                                                              const GroupChunk* __restrict__ os, GroupSide q) {

@@ -63,7 +63,7 @@ struct LkScal {
 
 // ---------------------------------------------------------------- scalars
 // v, a' and n_eff of every instance from the table of distinct counts (n of them sum to at least n(n-1)/2 positions: 1414
-// at 10^6 positions), one workgroup per instance.
+// at 10^6 positions), one workgroup per instance: a few us, bound by its latency, so it rides in a launch that is there anyway.
 struct LkScalArgs {
     const double* cnt;
     const double* az;
@@ -254,7 +254,7 @@ __global__ __launch_bounds__(kBlock) void lookup_apply_kernel(size_t V, size_t D
         if (t0 + i * G < n_pos) lk_store<T, ROW>(x + (b * n_pos + t0 + i * G) * D + k.col, k.valid, v[i]);
 }
 
-// one column: N positions per lane, written as one piece
+// one column: N positions per lane, written as one piece; bound by the gathers (64 x 100000 f64 of 200000: 53 us)
 template <typename T>
 __global__ __launch_bounds__(kBlock) void lookup_apply1_kernel(size_t V, size_t n_pos, double s, unsigned blocks, unsigned batch, int spread,
                                                                const int* __restrict__ tok, const T* __restrict__ z, T* __restrict__ x) {
@@ -431,7 +431,8 @@ __device__ __forceinline__ void lk_chunk(const LkArgs& a, const LkLane& k, size_
         if (e < k.valid) p[e] = acc[e];
 }
 
-// First launch: the partial sums of the heavy runs; one more workgroup per instance makes its scalars.
+// First launch: the partial sums of the heavy runs; one more workgroup per instance makes its scalars.  Bound by the read of their
+// positions: 622000 of 64 f32 (of 10^6 over 50000 rows, Zipf), 159 MB, 35 us, 4.6 TB/s.
 template <typename T, int ROW, bool ONCE>
 __global__ __launch_bounds__(kBlock) void lookup_chunks_kernel(LkArgs a, LkScalArgs q, const T* __restrict__ x, double* __restrict__ partials) {
     __shared__ double sm[kBlock / kWave][kWave][LkVec<T>::N];
@@ -447,6 +448,10 @@ __global__ __launch_bounds__(kBlock) void lookup_chunks_kernel(LkArgs a, LkScalA
 
 // Second launch: every run.  Workgroups, in this order: joins of the partial sums, block runs, wave runs, light ones.  The gradient
 // needs no scalars: with short rows its chunks lead this launch and only their joins are left for another.
+// Bound by the bytes where a row fills its lines: the other 378000 positions of that message, 207 MB read and written, 47 us,
+// 4.4 TB/s; gradient of 65536 x 1024 f32 to 32000 rows 246 MB 56 us, after 23 us for 110 MB of heavy runs.  Rows that share lines
+// are bound by the lines: 168 bytes touch 2.3 of 128 on average, message of 8 x 80021 x 21 f64 to 10007 rows 36 us; one column
+// by a line from the L2 per element, 8 bytes of 128: gradient of 1000001 f64 20 us.
 template <typename T, int ROW, int MODE, bool SELF>
 __global__ __launch_bounds__(kBlock) void lookup_rows_kernel(LkArgs a, LkScalArgs q, const LkScal* __restrict__ scal, const T* __restrict__ bz,
                                                              const T* __restrict__ x, double damping, const T* b_old, T* out,
@@ -623,7 +628,8 @@ __global__ __launch_bounds__(kBlock) void lookup_rows_kernel(LkArgs a, LkScalArg
 }
 
 // Third launch of the message to the positions: those of the heavy runs and the padded ones (slot -1: rx = 0), the chunks that were
-// summed last first - they are the likeliest to be cached still (10^6 x 64 f32: 150 us forwards, 138 us backwards).
+// summed last first - they are the likeliest to be cached still (10^6 x 64 f32: 150 us forwards, 138 us backwards).  Bound by
+// the write and what is read twice: 318 MB, 53 us, 6.0 TB/s.
 template <typename T, int ROW>
 __global__ __launch_bounds__(kBlock) void lookup_spread_kernel(LkArgs a, const LkItem* __restrict__ spreads, const LkScal* __restrict__ scal,
                                                                const double* __restrict__ sr_ws, const T* __restrict__ bx, double damping,
@@ -657,7 +663,9 @@ __global__ __launch_bounds__(kBlock) void lookup_spread_kernel(LkArgs a, const L
 // ---------------------------------------------------------------- the message to x in the order of the positions
 // Rows shorter than half a line cost a line each when they are read or written in the order of the tokens.  Here the sums of the
 // runs of two and more positions leave scale r in double (LK_MEAN), and x is walked in its own order: a position that is
-// alone in its run has its sum at hand, the others fetch theirs.  One column: a lane takes one 16-byte piece of positions.
+// alone in its run has its sum at hand, the others fetch theirs.  One column: a lane takes one 16-byte piece of positions.  Bound
+// by the lines a gather takes from the L2: 64 instances of 100000 positions of 200000 f64, 6.4 10^6 gathers, 52 us, and 41 us for
+// the sums before.  Runs of two and three summed at each of their positions instead: 102 us in all against 99.
 template <typename T, int ROW>
 __global__ __launch_bounds__(kBlock) void lookup_positions_kernel(LkArgs a, const int* __restrict__ code, const LkScal* __restrict__ scal,
                                                                   const T* __restrict__ bz, const double* __restrict__ sr_ws,
@@ -739,7 +747,8 @@ __global__ __launch_bounds__(kBlock) void lookup_positions1_kernel(LkArgs a, con
 }
 
 // ---------------------------------------------------------------- log-partition
-// A = 1/2 sum_v (bz + g)^2 / prec + D/2 sum_v log(2 pi / prec)   (linear_channel.py:127-132): the rows' shares, added in two steps
+// A = 1/2 sum_v (bz + g)^2 / prec + D/2 sum_v log(2 pi / prec)   (linear_channel.py:127-132): the rows' shares, one double per row
+// and column tile, added in two steps.  Once per run, not per iteration; bound like the message to the table.
 __global__ __launch_bounds__(kBlock) void lookup_fold_kernel(size_t n, const double* __restrict__ in, double* __restrict__ out) {
     __shared__ double smem[kBlock / kWave];
     const size_t b = blockIdx.y;
@@ -1159,6 +1168,8 @@ extern "C" int tramp_lookup_message(tramp_ctx* ctx, tramp_lookup* lk, int dir, s
     TRAMP_REQUIRE(ctx, !lk_overlap(b_new_d, no, bz_d, nz) && !lk_overlap(b_new_d, no, bx_d, nx));
     TRAMP_REQUIRE(ctx, !lk_overlap(r_d, no, bz_d, nz) && !lk_overlap(r_d, no, bx_d, nx) && !lk_overlap(r_d, no, b_new_d, no));
     TRAMP_REQUIRE(ctx, damping == 0.0 || b_old_d == b_new_d || !lk_overlap(b_old_d, no, b_new_d, no));
+    TRAMP_REQUIRE(ctx, damping == 0.0 || !lk_overlap(b_old_d, no, r_d, no));
+    TRAMP_REQUIRE(ctx, damping == 0.0 || !lk_overlap(b_old_d, no, r_d, no));
     TRAMP_REQUIRE(ctx, damping == 0.0 || (a_old_d && b_old_d));
     if (!batch) return TRAMP_OK;
     if (lk->dtype == TRAMP_F64)
