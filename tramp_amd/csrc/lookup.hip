@@ -177,6 +177,22 @@ __device__ __forceinline__ void lk_store(T* p, int valid, const T (&v)[LkVec<T>:
     }
 }
 
+// one column in its own order: pieces side by side past the caches, which are left to what is gathered (lookup of 64 x 100000 f64
+// 53.7 -> 49.9 us, of 10^6 7.2 -> 6.1; message to x by position of 64 x 100000 f64 99.1 -> 95.4 us, read so too; one instance, whose x
+// the sums have just read, 37.5 -> 38.5 if read so)
+template <typename T> __device__ __forceinline__ void lk_stream_load(const T* __restrict__ p, int valid, T (&v)[LkVec<T>::N]) {
+    if (valid == LkVec<T>::N)
+        lk_load<T, LK_LINES, true>(p, valid, v);
+    else
+        lk_load<T, LK_TAIL>(p, valid, v);
+}
+template <typename T> __device__ __forceinline__ void lk_stream_store(T* p, int valid, const T (&v)[LkVec<T>::N]) {
+    if (valid == LkVec<T>::N)
+        lk_store<T, LK_LINES>(p, valid, v);
+    else
+        lk_store<T, LK_TAIL>(p, valid, v);
+}
+
 // where a lane stands: its group (one row at a time per group), its piece of the row
 struct LkLane {
     int lw;                      // log2 LPR
@@ -254,7 +270,7 @@ __global__ __launch_bounds__(kBlock) void lookup_apply_kernel(size_t V, size_t D
         if (t0 + i * G < n_pos) lk_store<T, ROW>(x + (b * n_pos + t0 + i * G) * D + k.col, k.valid, v[i]);
 }
 
-// one column: N positions per lane, written as one piece; bound by the gathers (64 x 100000 f64 of 200000: 53 us)
+// one column: N positions per lane, written as one piece; bound by the gathers (64 x 100000 f64 of 200000: 50 us)
 template <typename T>
 __global__ __launch_bounds__(kBlock) void lookup_apply1_kernel(size_t V, size_t n_pos, double s, unsigned blocks, unsigned batch, int spread,
                                                                const int* __restrict__ tok, const T* __restrict__ z, T* __restrict__ x) {
@@ -269,7 +285,7 @@ __global__ __launch_bounds__(kBlock) void lookup_apply1_kernel(size_t V, size_t 
     for (int i = 0; i < N; ++i) row[i] = i < valid ? tok[t + i] : -1;
 #pragma unroll
     for (int i = 0; i < N; ++i) v[i] = row[i] >= 0 ? T(s * (double)z[b * V + (size_t)row[i]]) : T(0);
-    lk_store<T, LK_TAIL>(x + b * n_pos + t, valid, v);
+    lk_stream_store<T>(x + b * n_pos + t, valid, v);
 }
 
 // ---------------------------------------------------------------- sums over the runs
@@ -664,8 +680,9 @@ __global__ __launch_bounds__(kBlock) void lookup_spread_kernel(LkArgs a, const L
 // Rows shorter than half a line cost a line each when they are read or written in the order of the tokens.  Here the sums of the
 // runs of two and more positions leave scale r in double (LK_MEAN), and x is walked in its own order: a position that is
 // alone in its run has its sum at hand, the others fetch theirs.  One column: a lane takes one 16-byte piece of positions.  Bound
-// by the lines a gather takes from the L2: 64 instances of 100000 positions of 200000 f64, 6.4 10^6 gathers, 52 us, and 41 us for
-// the sums before.  Runs of two and three summed at each of their positions instead: 102 us in all against 99.
+// by the lines a gather takes from the L2: 64 instances of 100000 positions of 200000 f64, 6.4 10^6 gathers, 49 us, and 41 us for
+// the sums before.  Dropped: runs of two and three summed at each of their positions (102 us in all against 99), two pieces per lane
+// (100).
 template <typename T, int ROW>
 __global__ __launch_bounds__(kBlock) void lookup_positions_kernel(LkArgs a, const int* __restrict__ code, const LkScal* __restrict__ scal,
                                                                   const T* __restrict__ bz, const double* __restrict__ sr_ws,
@@ -726,7 +743,10 @@ __global__ __launch_bounds__(kBlock) void lookup_positions1_kernel(LkArgs a, con
 #pragma unroll
         for (int i = 0; i < N; ++i) w[i] = i < valid ? code[t + i] : -1;
     }
-    lk_load<T, LK_TAIL>(bx + b * a.T + t, valid, v);
+    if (a.spread)                                                  // the L2 is for the table of the instance
+        lk_stream_load<T>(bx + b * a.T + t, valid, v);
+    else
+        lk_load<T, LK_TAIL>(bx + b * a.T + t, valid, v);
     if (damping != 0.0) lk_load<T, LK_TAIL>(b_old + b * a.T + t, valid, old);
 #pragma unroll
     for (int i = 0; i < N; ++i)
@@ -738,7 +758,7 @@ __global__ __launch_bounds__(kBlock) void lookup_positions1_kernel(LkArgs a, con
         if (damping != 0.0) m = damping * (double)old[i] + (1.0 - damping) * m;
         o[i] = T(m);
     }
-    lk_store<T, LK_TAIL>(out + b * a.T + t, valid, o);
+    lk_stream_store<T>(out + b * a.T + t, valid, o);
     if (r_out) {
 #pragma unroll
         for (int i = 0; i < N; ++i) o[i] = T(z[i]);
