@@ -680,7 +680,7 @@ __global__ __launch_bounds__(kBlock) void lookup_spread_kernel(LkArgs a, const L
 // Rows shorter than half a line cost a line each when they are read or written in the order of the tokens.  Here the sums of the
 // runs of two and more positions leave scale r in double (LK_MEAN), and x is walked in its own order: a position that is
 // alone in its run has its sum at hand, the others fetch theirs.  One column: a lane takes one 16-byte piece of positions.  Bound
-// by the lines a gather takes from the L2: 64 instances of 100000 positions of 200000 f64, 6.4 10^6 gathers, 49 us, and 41 us for
+// by the lines a gather takes from the L2: 64 instances of 100000 positions of 200000 f64, 6.4 10^6 gathers, 44 us, and 37 us for
 // the sums before.  Dropped: runs of two and three summed at each of their positions (102 us in all against 99), two pieces per lane
 // (100).
 template <typename T, int ROW>
