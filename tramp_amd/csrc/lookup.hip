@@ -46,10 +46,11 @@ struct tramp_lookup {
     const LkItem* runs;          // runs for one workgroup
     const LkItem* waves;         // runs for one wave
     const LkItem* light;         // the shorter runs, by falling length; slot: the first position
+    const int* empty;            // rows without positions
     const int* idx;              // [V] place among the runs of two and more positions (short rows only)
     const int* code;             // [T] that place, -1 where padded, -2 - token where the run is this position (short rows only)
     int K;
-    unsigned n_chunks, n_joins, n_spreads, n_runs, n_waves, n_light, n_light2, n_multi;
+    unsigned n_chunks, n_joins, n_spreads, n_runs, n_waves, n_light, n_light2, n_empty, n_multi;
     int lw;                      // log2 of the lanes per row
     unsigned tiles;              // column tiles per row
     int row;                     // LK_TAIL / LK_WHOLE / LK_LINES
@@ -300,6 +301,10 @@ __global__ __launch_bounds__(kBlock) void lookup_apply1_kernel(size_t V, size_t 
 // kKeep: 8 rows in flight per group leave 5 to 8 waves per SIMD; 16 leave 3 to 5 and cost a third (gradient 121 against 84 us,
 // message to 10^6 positions of 64 columns 136 against 104 us), 4 make longer runs of every kind (89 and 103 us).
 constexpr int kKeep = 8;
+// Rows that no position reads (most rows of a table of many, in a batch of few) have a kind of their own, four per group, and the
+// others come from the list, unless rows are short and want to be written side by side.  Gradient of 65536 x 1024 f32 to 32000 rows
+// (20600 without positions) 78.6 -> 69.3 us, 133588 x 76 f64 to 172932 rows 105 -> 77, 8 x 201 x 71 f32 to 68544 rows 75 -> 40.
+constexpr int kEmpty = 4;
 
 struct LkArgs {
     const int* off;
@@ -309,9 +314,10 @@ struct LkArgs {
     const LkItem* runs;
     const LkItem* waves;
     const LkItem* light;         // null: all rows of the table (those of the kinds above left out)
+    const int* empty;
     const int* idx;
     size_t V, D, T;
-    unsigned n_chunks, n_joins, n_runs, n_waves, wave_blocks, n_light, n_multi, blocks, tiles, batch;
+    unsigned n_chunks, n_joins, n_runs, n_waves, wave_blocks, n_light, light_blocks, n_empty, n_multi, blocks, tiles, batch;
     unsigned n_lead;             // chunks summed in the launch of the runs (gradient)
     int lw, spread;
     double s;
@@ -542,6 +548,21 @@ __global__ __launch_bounds__(kBlock) void lookup_rows_kernel(LkArgs a, LkScalArg
             sub = (threadIdx.x & 63) >> a.lw;
             ls = 6 - a.lw;
             first = (threadIdx.x & 63) < (1u << a.lw);
+        } else if ((MODE == LK_GRAD || MODE == LK_BWD) && blk >= a.wave_blocks + a.light_blocks) {
+            // rows that no position reads, four per group: the table alone makes their result
+            const size_t G = kBlock >> a.lw, u0 = (size_t)(blk - a.wave_blocks - a.light_blocks) * kEmpty * G + k.group;
+            int row[kEmpty];
+            T zs[kEmpty][N];
+            if (!act) return;
+#pragma unroll
+            for (int i = 0; i < kEmpty; ++i) row[i] = u0 + i * G < a.n_empty ? a.empty[u0 + i * G] : -1;
+#pragma unroll
+            for (int i = 0; i < kEmpty; ++i)
+                if (MODE == LK_BWD && row[i] >= 0) lk_load<T, ROW, true>(bz + (b * a.V + (size_t)row[i]) * a.D + k.col, k.valid, zs[i]);
+#pragma unroll
+            for (int i = 0; i < kEmpty; ++i)
+                if (row[i] >= 0) lk_row_out<T, ROW, MODE>(a, c, k, b, row[i], 0, acc, zs[i], damping, b_old, out, r_out);
+            return;
         } else {
             const size_t u = (size_t)(blk - a.wave_blocks) * (kBlock >> a.lw) + k.group;
             if (u >= a.n_light) return;
@@ -817,11 +838,12 @@ extern "C" int tramp_lookup_create(tramp_ctx* ctx, int dtype, size_t n_rows, siz
         const int per_wave = kKeep << (6 - lw), per_block = kKeep << (8 - lw);
         const bool short_rows = n_cols * e < 64;
         std::vector<LkItem> chunks, runs, joins, spreads, waves, light, single;
-        std::vector<int> idx, code;
+        std::vector<int> idx, code, empty;
         for (size_t v = 0; v < n_rows; ++v) {
             const int c = counts[v], j0 = off[v];
-            if (c == 0) continue;
-            if (c == 1) {
+            if (c == 0) {
+                empty.push_back((int)v);
+            } else if (c == 1) {
                 single.push_back(LkItem{(int)v, j0, j0 + c, perm[(size_t)j0]});
             } else if (c <= kKeep) {
                 light.push_back(LkItem{(int)v, j0, j0 + c, perm[(size_t)j0]});
@@ -871,7 +893,7 @@ extern "C" int tramp_lookup_create(tramp_ctx* ctx, int dtype, size_t n_rows, siz
         cval.insert(cval.end(), cmul.begin(), cmul.end());
         // one allocation: the arrays one behind the other
         std::vector<char> host;
-        host.reserve(n_pos * (short_rows ? 12 : 8) + n_rows * (short_rows ? 8 : 4) + 2 * K * 8 + 16 * 256 +
+        host.reserve(n_pos * (short_rows ? 12 : 8) + n_rows * (short_rows ? 8 : 4) + empty.size() * 4 + 2 * K * 8 + 16 * 256 +
                      sizeof(LkItem) * (chunks.size() + joins.size() + spreads.size() + runs.size() + waves.size() + light.size()));
         auto put = [&host](const void* p, size_t bytes) {
             const size_t at = host.size();
@@ -884,6 +906,7 @@ extern "C" int tramp_lookup_create(tramp_ctx* ctx, int dtype, size_t n_rows, siz
         const size_t o_joins = put(joins.data(), joins.size() * sizeof(LkItem)), o_spreads = put(spreads.data(), spreads.size() * sizeof(LkItem));
         const size_t o_runs = put(runs.data(), runs.size() * sizeof(LkItem)), o_waves = put(waves.data(), waves.size() * sizeof(LkItem));
         const size_t o_light = put(light.data(), light.size() * sizeof(LkItem)), o_idx = put(idx.data(), idx.size() * 4), o_code = put(code.data(), code.size() * 4);
+        const size_t o_empty = put(empty.data(), empty.size() * 4);
         tramp_lookup* lk = new tramp_lookup();
         *lk = tramp_lookup{};
         (void)hipSetDevice(ctx->device);
@@ -919,6 +942,8 @@ extern "C" int tramp_lookup_create(tramp_ctx* ctx, int dtype, size_t n_rows, siz
         lk->light = reinterpret_cast<const LkItem*>(m + o_light);
         lk->idx = reinterpret_cast<const int*>(m + o_idx);
         lk->code = reinterpret_cast<const int*>(m + o_code);
+        lk->empty = reinterpret_cast<const int*>(m + o_empty);
+        lk->n_empty = (unsigned)empty.size();
         lk->K = (int)K;
         lk->n_chunks = (unsigned)chunks.size();
         lk->n_joins = (unsigned)joins.size();
@@ -1060,7 +1085,9 @@ static int launch_rows(tramp_ctx* ctx, const tramp_lookup* lk, size_t batch, con
     a.joins = lk->joins;
     a.runs = lk->runs;
     a.waves = lk->waves;
-    a.light = MODE == LK_FWD || MODE == LK_MEAN ? lk->light : nullptr;
+    const bool listed = MODE == LK_FWD || MODE == LK_MEAN || ((MODE == LK_GRAD || MODE == LK_BWD) && !lk->short_rows);
+    a.light = listed ? lk->light : nullptr;
+    a.empty = lk->empty;
     a.idx = lk->idx;
     a.V = lk->V;
     a.D = lk->D;
@@ -1070,7 +1097,8 @@ static int launch_rows(tramp_ctx* ctx, const tramp_lookup* lk, size_t batch, con
     a.n_runs = lk->n_runs;
     a.n_waves = lk->n_waves;
     a.wave_blocks = (lk->n_waves + kBlock / kWave - 1) / (kBlock / kWave);
-    a.n_light = MODE == LK_FWD ? lk->n_light : MODE == LK_MEAN ? lk->n_light2 : (unsigned)lk->V;
+    a.n_light = MODE == LK_MEAN ? lk->n_light2 : listed ? lk->n_light : (unsigned)lk->V;
+    a.n_empty = listed && (MODE == LK_GRAD || MODE == LK_BWD) ? lk->n_empty : 0;
     a.n_multi = lk->n_multi;
     a.tiles = lk->tiles;
     a.batch = (unsigned)batch;
@@ -1081,7 +1109,8 @@ static int launch_rows(tramp_ctx* ctx, const tramp_lookup* lk, size_t batch, con
     // would lose: 65536 x 1024 f32 78.7 against 83.1 us, 20000 x 300 f64 15.2 against 16.1
     a.n_lead = MODE == LK_GRAD && lk->short_rows ? lk->n_chunks : 0;
     if (a.n_lead) a.n_joins = 0;
-    const size_t blocks = (size_t)a.n_lead + a.n_joins + a.n_runs + a.wave_blocks + ((size_t)a.n_light + G - 1) / G;
+    a.light_blocks = (unsigned)(((size_t)a.n_light + G - 1) / G);
+    const size_t blocks = (size_t)a.n_lead + a.n_joins + a.n_runs + a.wave_blocks + a.light_blocks + (a.n_empty + kEmpty * G - 1) / (kEmpty * G);
     TRAMP_REQUIRE(ctx, blocks * lk->tiles < 0x7fffffffu && (size_t)lk->n_spreads * lk->tiles < 0x7fffffffu &&
                            (size_t)lk->n_chunks * lk->tiles < 0x7ffffffeu);
     a.blocks = (unsigned)blocks;
@@ -1103,7 +1132,7 @@ static int launch_rows(tramp_ctx* ctx, const tramp_lookup* lk, size_t batch, con
     if (a.n_lead) {
         LkArgs j = a;
         j.n_joins = j.blocks = lk->n_joins;
-        j.n_lead = j.n_runs = j.n_waves = j.wave_blocks = j.n_light = 0;
+        j.n_lead = j.n_runs = j.n_waves = j.wave_blocks = j.n_light = j.light_blocks = j.n_empty = 0;
         j.spread = 0;
         hipLaunchKernelGGL((lookup_rows_kernel<T, ROW, MODE, false>), lk_grid(batch, (size_t)j.blocks * lk->tiles, 0), dim3(kBlock), 0, ctx->stream,
                            j, LkScalArgs{}, w.scal, bz, x, damping, b_old, out, r_out, w.partials, w.sr);
