@@ -291,7 +291,7 @@ __global__ __launch_bounds__(kBlock) void lookup_apply1_kernel(size_t V, size_t 
 
 // ---------------------------------------------------------------- sums over the runs
 // The run lengths of real tokens differ by orders of magnitude, so the work is cut by them, at creation:
-//   light  run <= kKeep                       one group, all rows of the run in flight at once
+//   light  run <= kKeep                       one group, all rows of the run in flight at once (of none or one position: below)
 //   wave   run <= kKeep * 64 / LPR            the groups of one wave, joined by a butterfly
 //   block  run <= kKeep * 256 / LPR           the groups of one workgroup, the four waves joined through LDS
 //   heavy  longer                             chunks of a multiple of that, summed in a first launch (lookup_chunks_kernel),
@@ -305,6 +305,9 @@ constexpr int kKeep = 8;
 // others come from the list, unless rows are short and want to be written side by side.  Gradient of 65536 x 1024 f32 to 32000 rows
 // (20600 without positions) 78.6 -> 69.3 us, 133588 x 76 f64 to 172932 rows 105 -> 77, 8 x 201 x 71 f32 to 68544 rows 75 -> 40.
 constexpr int kEmpty = 4;
+// Rows that one position reads, two per group: gradient of 133588 x 76 f64 to 172932 rows 76.9 -> 70.8 us, the message to that table
+// 96.4 -> 84.9, to those positions 99.8 -> 77.6.  Four cost registers: 68.5, 92.9 and 77.0, but message to 8 x 10007 x 21 f64 46 -> 50.
+constexpr int kOne = 2;
 
 struct LkArgs {
     const int* off;
@@ -317,7 +320,7 @@ struct LkArgs {
     const int* empty;
     const int* idx;
     size_t V, D, T;
-    unsigned n_chunks, n_joins, n_runs, n_waves, wave_blocks, n_light, light_blocks, n_empty, n_multi, blocks, tiles, batch;
+    unsigned n_chunks, n_joins, n_runs, n_waves, wave_blocks, n_light, light_blocks, n_single, single_blocks, n_empty, n_multi, blocks, tiles, batch;
     unsigned n_lead;             // chunks summed in the launch of the runs (gradient)
     int lw, spread;
     double s;
@@ -468,7 +471,8 @@ __global__ __launch_bounds__(kBlock) void lookup_chunks_kernel(LkArgs a, LkScalA
     lk_chunk<T, ROW, ONCE>(a, k, b, blk, x + b * a.T * a.D, partials, sm);
 }
 
-// Second launch: every run.  Workgroups, in this order: joins of the partial sums, block runs, wave runs, light ones.  The gradient
+// Second launch: every run.  Workgroups, in this order: joins of the partial sums, block runs, wave runs, light ones,
+// rows of one position, rows of none.  The gradient
 // needs no scalars: with short rows its chunks lead this launch and only their joins are left for another.
 // Bound by the bytes where a row fills its lines: the other 378000 positions of that message, 207 MB read and written, 47 us,
 // 4.4 TB/s; gradient of 65536 x 1024 f32 to 32000 rows 246 MB 56 us, after 23 us for 110 MB of heavy runs.  Rows that share lines
@@ -548,9 +552,40 @@ __global__ __launch_bounds__(kBlock) void lookup_rows_kernel(LkArgs a, LkScalArg
             sub = (threadIdx.x & 63) >> a.lw;
             ls = 6 - a.lw;
             first = (threadIdx.x & 63) < (1u << a.lw);
+        } else if ((MODE == LK_GRAD || MODE == LK_BWD || MODE == LK_FWD) && blk >= a.wave_blocks + a.light_blocks &&
+                   blk < a.wave_blocks + a.light_blocks + a.single_blocks) {
+            // rows that one position reads, two per group
+            const size_t G = kBlock >> a.lw, u0 = (size_t)(blk - a.wave_blocks - a.light_blocks) * kOne * G + k.group;
+            LkItem it[kOne];
+            T xs[kOne][N], zs[kOne][N];
+            if (!act) return;
+#pragma unroll
+            for (int i = 0; i < kOne; ++i) it[i] = u0 + i * G < a.n_single ? a.light[a.n_light + u0 + i * G] : LkItem{-1, 0, 0, 0};
+#pragma unroll
+            for (int i = 0; i < kOne; ++i)
+                if (it[i].token >= 0) {
+                    lk_load<T, ROW, true>(xb + (size_t)it[i].slot * a.D + k.col, k.valid, xs[i]);
+                    if (MODE != LK_GRAD) lk_load<T, ROW, MODE == LK_BWD>(bz + (b * a.V + (size_t)it[i].token) * a.D + k.col, k.valid, zs[i]);
+                }
+            const double f = a.s / (c.az + c.lik1);
+#pragma unroll
+            for (int i = 0; i < kOne; ++i) {
+                if (it[i].token < 0) continue;
+                if (MODE == LK_FWD) {
+                    double sr[N];
+#pragma unroll
+                    for (int e = 0; e < N; ++e) sr[e] = f * ((double)zs[i][e] + a.s * (0.0 + (double)xs[i][e]));
+                    lk_position_out<T, ROW>(a, c.ax + c.an, k, b, (size_t)it[i].slot, sr, xs[i], damping, b_old, out, r_out);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < N; ++e) acc[e] = 0.0 + (double)xs[i][e];
+                    lk_row_out<T, ROW, MODE>(a, c, k, b, it[i].token, 1, acc, zs[i], damping, b_old, out, r_out);
+                }
+            }
+            return;
         } else if ((MODE == LK_GRAD || MODE == LK_BWD) && blk >= a.wave_blocks + a.light_blocks) {
             // rows that no position reads, four per group: the table alone makes their result
-            const size_t G = kBlock >> a.lw, u0 = (size_t)(blk - a.wave_blocks - a.light_blocks) * kEmpty * G + k.group;
+            const size_t G = kBlock >> a.lw, u0 = (size_t)(blk - a.wave_blocks - a.light_blocks - a.single_blocks) * kEmpty * G + k.group;
             int row[kEmpty];
             T zs[kEmpty][N];
             if (!act) return;
@@ -1097,7 +1132,8 @@ static int launch_rows(tramp_ctx* ctx, const tramp_lookup* lk, size_t batch, con
     a.n_runs = lk->n_runs;
     a.n_waves = lk->n_waves;
     a.wave_blocks = (lk->n_waves + kBlock / kWave - 1) / (kBlock / kWave);
-    a.n_light = MODE == LK_MEAN ? lk->n_light2 : listed ? lk->n_light : (unsigned)lk->V;
+    a.n_light = listed ? lk->n_light2 : (unsigned)lk->V;
+    a.n_single = listed && MODE != LK_MEAN ? lk->n_light - lk->n_light2 : 0;
     a.n_empty = listed && (MODE == LK_GRAD || MODE == LK_BWD) ? lk->n_empty : 0;
     a.n_multi = lk->n_multi;
     a.tiles = lk->tiles;
@@ -1110,7 +1146,8 @@ static int launch_rows(tramp_ctx* ctx, const tramp_lookup* lk, size_t batch, con
     a.n_lead = MODE == LK_GRAD && lk->short_rows ? lk->n_chunks : 0;
     if (a.n_lead) a.n_joins = 0;
     a.light_blocks = (unsigned)(((size_t)a.n_light + G - 1) / G);
-    const size_t blocks = (size_t)a.n_lead + a.n_joins + a.n_runs + a.wave_blocks + a.light_blocks + (a.n_empty + kEmpty * G - 1) / (kEmpty * G);
+    a.single_blocks = (unsigned)((a.n_single + kOne * G - 1) / (kOne * G));
+    const size_t blocks = (size_t)a.n_lead + a.n_joins + a.n_runs + a.wave_blocks + a.light_blocks + a.single_blocks + (a.n_empty + kEmpty * G - 1) / (kEmpty * G);
     TRAMP_REQUIRE(ctx, blocks * lk->tiles < 0x7fffffffu && (size_t)lk->n_spreads * lk->tiles < 0x7fffffffu &&
                            (size_t)lk->n_chunks * lk->tiles < 0x7ffffffeu);
     a.blocks = (unsigned)blocks;
@@ -1132,7 +1169,7 @@ static int launch_rows(tramp_ctx* ctx, const tramp_lookup* lk, size_t batch, con
     if (a.n_lead) {
         LkArgs j = a;
         j.n_joins = j.blocks = lk->n_joins;
-        j.n_lead = j.n_runs = j.n_waves = j.wave_blocks = j.n_light = j.light_blocks = j.n_empty = 0;
+        j.n_lead = j.n_runs = j.n_waves = j.wave_blocks = j.n_light = j.light_blocks = j.n_single = j.single_blocks = j.n_empty = 0;
         j.spread = 0;
         hipLaunchKernelGGL((lookup_rows_kernel<T, ROW, MODE, false>), lk_grid(batch, (size_t)j.blocks * lk->tiles, 0), dim3(kBlock), 0, ctx->stream,
                            j, LkScalArgs{}, w.scal, bz, x, damping, b_old, out, r_out, w.partials, w.sr);
