@@ -471,13 +471,13 @@ __global__ __launch_bounds__(kBlock) void lookup_chunks_kernel(LkArgs a, LkScalA
     lk_chunk<T, ROW, ONCE>(a, k, b, blk, x + b * a.T * a.D, partials, sm);
 }
 
-// Second launch: every run.  Workgroups, in this order: joins of the partial sums, block runs, wave runs, light ones,
-// rows of one position, rows of none.  The gradient
-// needs no scalars: with short rows its chunks lead this launch and only their joins are left for another.
+// Second launch: every run.  Workgroups, in this order: joins of the partial sums, block runs, wave runs, light ones, rows of one
+// position, rows of none.  The gradient needs no scalars: with short rows its chunks lead this launch and only their joins are
+// left for another.
 // Bound by the bytes where a row fills its lines: the other 378000 positions of that message, 207 MB read and written, 47 us,
-// 4.4 TB/s; gradient of 65536 x 1024 f32 to 32000 rows 246 MB 56 us, after 23 us for 110 MB of heavy runs.  Rows that share lines
-// are bound by the lines: 168 bytes touch 2.3 of 128 on average, message of 8 x 80021 x 21 f64 to 10007 rows 36 us; one column
-// by a line from the L2 per element, 8 bytes of 128: gradient of 1000001 f64 20 us.
+// 4.4 TB/s; gradient of 65536 x 1024 f32 to 32000 rows 246 MB 46 us, 5.3 TB/s, after 23 us for 110 MB of heavy runs.  Rows that
+// share lines are bound by the lines: 168 bytes touch 2.3 of 128 on average, message of 8 x 80021 x 21 f64 to 10007 rows 34 us;
+// one column by a line from the L2 per element, 8 bytes of 128: gradient of 1000001 f64 17 us.
 template <typename T, int ROW, int MODE, bool SELF>
 __global__ __launch_bounds__(kBlock) void lookup_rows_kernel(LkArgs a, LkScalArgs q, const LkScal* __restrict__ scal, const T* __restrict__ bz,
                                                              const T* __restrict__ x, double damping, const T* b_old, T* out,
