@@ -281,7 +281,8 @@ def test_captured_calls_replay_and_share_workspaces(ctx):
 
 @pytest.mark.parametrize("V, n, D, B, zipf, pad, dtype", [(700001, 600000, 1, 1, None, 0.0, np.float64), (3000, 90000, 7, 1, 1.1, 0.1, np.float64),
                                                           (500, 80000, 1, 16, 1.0, 0.2, np.float32), (2500, 40001, 3, 16, 1.2, 0.1, np.float32),
-                                                          (20000, 30000, 5, 8, 0.5, 0.0, np.float64), (300, 200000, 33, 3, 1.0, 0.1, np.float32)])
+                                                          (20000, 30000, 5, 8, 0.5, 0.0, np.float64), (300, 200000, 33, 3, 1.0, 0.1, np.float32),
+                                                          (9001, 3001, 40, 3, 0.3, 0.1, np.float64), (6000, 2501, 96, 8, 0.0, 0.0, np.float32)])
 def test_larger_messages(ctx, V, n, D, B, zipf, pad, dtype):
     "the forms that only larger calls take: by position, heavy runs, instances by XCD, no token twice; same tolerances"
     import tramp_amd as T
@@ -313,6 +314,43 @@ def test_larger_messages(ctx, V, n, D, B, zipf, pad, dtype):
             # b' = r (a + a') - b on the posterior the same call gives, which is rounded once more
             lim = k * mag + eps2(dtype) * (np.abs(rb) + np.abs(R[i].astype(float)) * (a_in + ra)) + 4 * U * (np.abs(R[i].astype(float)) * (a_in + ra) + np.abs(own))
             assert (np.abs(Bn[i] - (R[i].astype(float) * (a_in + ra) - own)) <= lim).all()
+
+
+@pytest.mark.parametrize("dtype", [np.float64, np.float32])
+@pytest.mark.parametrize("V, n, D, pad", [(5003, 1201, 33, 0.1), (1203, 2001, 64, 0.0), (70, 9, 1030, 0.3), (9, 9, 16, 0.0), (4001, 3, 17, 0.0), (3001, 40, 1, 0.0),
+                                          (6, 5, 130, 1.0)])
+def test_rows_that_few_positions_read(ctx, V, n, D, pad, dtype):
+    "tables of rows read once or never: every component is written, and the sums of one position are that position's"
+    import tramp_amd as T
+    rs = np.random.RandomState(V + n)
+    tok = zipf_tokens(rs, V, n, 0.2, pad)
+    ch, ref = T.LookupChannel(tok, V, dim=D, scale=-0.6, padding_index=-1, dtype=dtype, ctx=ctx), LookupFactor(tok, V, D, -0.6)
+    B = 2
+    z, x = rs.standard_normal((B, V * D)).astype(dtype), rs.standard_normal((B, n * D)).astype(dtype)
+    unset = lambda m: ctx.array(np.full((B, m), np.nan), dtype)            # noqa: E731
+    G = ch.gradient(ctx.array(x, dtype), out=unset(V * D)).get()
+    plain = LookupFactor(tok, V, D, 1.0)
+    az, ax = np.array([0.8, 5.0]), np.array([2.0, 0.1])
+    args = ctx.scalars(az), ctx.array(z, dtype), ctx.scalars(ax), ctx.array(x, dtype)
+    k = 2 * (ref.count.max() + 2 * np.unique(ref.count).size + 32) * U
+    for b in range(B):
+        want = ref.gradient(x[b]).reshape(-1)
+        mag = 0.6 * plain.gradient(np.abs(x[b])).reshape(-1)
+        assert (np.abs(G[b] - want) <= eps2(dtype) * np.abs(want) + 2 * (ref.count.max() + 2) * U * mag).all()
+    assert (G.reshape(B, V, D)[:, ref.count == 0] == 0).all()
+    for direction, m in (("forward", n * D), ("backward", V * D)):
+        got = getattr(ch, f"compute_{direction}_message")(*args, out_a=ctx.scalars(np.ones(B)), out_b=unset(m))[1].get()
+        b0 = rs.standard_normal((B, m)).astype(dtype)
+        old = ctx.array(b0, dtype)
+        damped = getattr(ch, f"compute_{direction}_message")(*args, out_a=ctx.scalars(np.ones(B)), out_b=unset(m), damping=0.4,
+                                                             old_a=ctx.scalars(np.ones(B)), old_b=old)[1].get()
+        assert np.array_equal(old.get(), b0)
+        for b in range(B):
+            ra, rb = getattr(ref, direction)(az[b], z[b], ax[b], x[b])
+            mag = magnitudes(ref, az[b], z[b], ax[b], x[b], ra, direction)
+            assert (np.abs(got[b] - rb) <= eps2(dtype) * np.abs(rb) + k * mag).all()
+            want = 0.4 * b0[b].astype(float) + 0.6 * rb
+            assert (np.abs(damped[b] - want) <= eps2(dtype) * np.abs(want) + k * (mag + np.abs(b0[b]))).all()
 
 
 def test_a_precision_that_is_nan_stays_one(ctx):
