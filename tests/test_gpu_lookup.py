@@ -20,7 +20,8 @@ U = 2.0**-53
 SHAPES = [(1, 1, 1, 0.0, 0.0), (1, 5, 3, 0.0, 0.0), (7, 1, 1, 0.0, 0.0), (50, 200, 1, 1.0, 0.1), (33, 257, 5, 1.0, 0.2),
           (64, 1000, 64, 1.0, 0.0), (10, 5000, 16, 0.5, 0.05), (1000, 10, 4, 0.0, 0.0), (3, 20011, 2, 0.3, 0.0),
           (1, 70001, 1, 0.0, 0.5), (300, 900, 260, 1.2, 0.0), (40, 300, 1030, 1.0, 0.3), (4099, 30011, 1, 1.1, 0.0),
-          (20, 4, 8, 0.0, 1.0), (513, 2048, 12, 0.8, 0.0), (2, 9000, 130, 0.0, 0.0)]
+          (20, 4, 8, 0.0, 1.0), (513, 2048, 12, 0.8, 0.0), (2, 9000, 130, 0.0, 0.0),
+          (20, 177, 107, 0.9, 0.1), (2, 90, 260, 0.0, 0.0), (3, 150, 1100, 0.1, 0.0), (9, 2000, 18, 0.0, 0.2)]
 
 
 def make(T, ctx, shape, dtype, batch, scale, seed=0):
@@ -282,7 +283,8 @@ def test_captured_calls_replay_and_share_workspaces(ctx):
 @pytest.mark.parametrize("V, n, D, B, zipf, pad, dtype", [(700001, 600000, 1, 1, None, 0.0, np.float64), (3000, 90000, 7, 1, 1.1, 0.1, np.float64),
                                                           (500, 80000, 1, 16, 1.0, 0.2, np.float32), (2500, 40001, 3, 16, 1.2, 0.1, np.float32),
                                                           (20000, 30000, 5, 8, 0.5, 0.0, np.float64), (300, 200000, 33, 3, 1.0, 0.1, np.float32),
-                                                          (9001, 3001, 40, 3, 0.3, 0.1, np.float64), (6000, 2501, 96, 8, 0.0, 0.0, np.float32)])
+                                                          (9001, 3001, 40, 3, 0.3, 0.1, np.float64), (6000, 2501, 96, 8, 0.0, 0.0, np.float32),
+                                                          (500, 20000, 66, 8, 0.0, 0.05, np.float32), (300, 12000, 140, 5, 0.0, 0.0, np.float64)])
 def test_larger_messages(ctx, V, n, D, B, zipf, pad, dtype):
     "the forms that only larger calls take: by position, heavy runs, instances by XCD, no token twice; same tolerances"
     import tramp_amd as T

@@ -55,6 +55,7 @@ struct tramp_lookup {
     unsigned tiles;              // column tiles per row
     int row;                     // LK_TAIL / LK_WHOLE / LK_LINES
     bool short_rows;             // under half a line: the message to x may go in the order of the positions
+    bool long_runs;              // runs of one workgroup that its registers do not hold
 };
 
 // what the kernels need of one instance, written by lk_scalars
@@ -293,7 +294,7 @@ __global__ __launch_bounds__(kBlock) void lookup_apply1_kernel(size_t V, size_t 
 // The run lengths of real tokens differ by orders of magnitude, so the work is cut by them, at creation:
 //   light  run <= kKeep                       one group, all rows of the run in flight at once (of none or one position: below)
 //   wave   run <= kKeep * 64 / LPR            the groups of one wave, joined by a butterfly
-//   block  run <= kKeep * 256 / LPR           the groups of one workgroup, the four waves joined through LDS
+//   block  run <= kKeep * 256 / LPR           the groups of one workgroup, the four waves joined through LDS (LONG: twice that)
 //   heavy  longer                             chunks of a multiple of that, summed in a first launch (lookup_chunks_kernel),
 //                                             the partial sums in double joined by one workgroup in the second
 // In the first three every row stays in registers from the sum to the message that goes back to its position: the message to
@@ -478,7 +479,7 @@ __global__ __launch_bounds__(kBlock) void lookup_chunks_kernel(LkArgs a, LkScalA
 // 4.4 TB/s; gradient of 65536 x 1024 f32 to 32000 rows 246 MB 46 us, 5.3 TB/s, after 23 us for 110 MB of heavy runs.  Rows that
 // share lines are bound by the lines: 168 bytes touch 2.3 of 128 on average, message of 8 x 80021 x 21 f64 to 10007 rows 34 us;
 // one column by a line from the L2 per element, 8 bytes of 128: gradient of 1000001 f64 17 us.
-template <typename T, int ROW, int MODE, bool SELF>
+template <typename T, int ROW, int MODE, bool SELF, bool LONG>
 __global__ __launch_bounds__(kBlock) void lookup_rows_kernel(LkArgs a, LkScalArgs q, const LkScal* __restrict__ scal, const T* __restrict__ bz,
                                                              const T* __restrict__ x, double damping, const T* b_old, T* out,
                                                              T* __restrict__ r_out, double* __restrict__ partials,
@@ -537,7 +538,7 @@ __global__ __launch_bounds__(kBlock) void lookup_rows_kernel(LkArgs a, LkScalArg
         sub = k.group;
         ls = 8 - a.lw;
         first = threadIdx.x < (1u << a.lw);
-        if (act) lk_gather<T, ROW, kKeep, true, true>(a, xb, k, j0, count, sub, ls, p0, acc, pj, rows);
+        if (act) lk_gather<T, ROW, kKeep, MODE == LK_FWD && !LONG, true>(a, xb, k, j0, count, sub, ls, p0, acc, pj, rows);
         lk_block_join<N>(k, acc, sm);
     } else {
         blk -= a.n_runs;
@@ -694,6 +695,19 @@ __global__ __launch_bounds__(kBlock) void lookup_rows_kernel(LkArgs a, LkScalArg
         return;
     }
     const int cnt = count > sub ? ((count - sub - 1) >> ls) + 1 : 0;
+    if (LONG && ls == 8 - a.lw && count > kKeep << ls) {           // more than stayed in the registers
+        for (int j = 0; j < cnt; j += 4) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) pj[i] = j + i < cnt ? a.perm[j0 + sub + ((j + i) << ls)] : -1;
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (pj[i] >= 0) lk_load<T, ROW>(xb + (size_t)pj[i] * a.D + k.col, k.valid, rows[i]);
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (pj[i] >= 0) lk_position_out<T, ROW>(a, c.ax + c.an, k, b, (size_t)pj[i], sr, rows[i], damping, b_old, out, r_out);
+        }
+        return;
+    }
 #pragma unroll
     for (int i = 0; i < kKeep; ++i)
         if (i < cnt) lk_position_out<T, ROW>(a, c.ax + c.an, k, b, (size_t)pj[i], sr, rows[i], damping, b_old, out, r_out);
@@ -872,6 +886,12 @@ extern "C" int tramp_lookup_create(tramp_ctx* ctx, int dtype, size_t n_rows, siz
         const size_t tiles = (pieces + ((size_t)1 << lw) - 1) >> lw;
         const int per_wave = kKeep << (6 - lw), per_block = kKeep << (8 - lw);
         const bool short_rows = n_cols * e < 64;
+        // Runs of one workgroup: what its registers hold, or twice that where it spares the two launches of heavy runs: 2 x 177 x 107
+        // f64, V = 20: message to x 14.0 -> 9.2 us, gradient 8.1 -> 5.2; 8 x 20000 x 256 f32, V = 500: 105 -> 98, 45 -> 29.  Four times
+        // would leave too few workgroups: 7000 x 256 f32, V = 80, message to x 15.6 -> 17.9, 25000, V = 300: 23 -> 33.
+        const int most_read = *std::max_element(counts.begin(), counts.end());
+        const bool long_runs = most_read > per_block && most_read <= 2 * per_block;
+        const int longest = long_runs ? most_read : per_block;
         std::vector<LkItem> chunks, runs, joins, spreads, waves, light, single;
         std::vector<int> idx, code, empty;
         for (size_t v = 0; v < n_rows; ++v) {
@@ -884,7 +904,7 @@ extern "C" int tramp_lookup_create(tramp_ctx* ctx, int dtype, size_t n_rows, siz
                 light.push_back(LkItem{(int)v, j0, j0 + c, perm[(size_t)j0]});
             } else if (c <= per_wave) {
                 waves.push_back(LkItem{(int)v, j0, j0 + c, -1});
-            } else if (c <= per_block) {
+            } else if (c <= longest) {
                 runs.push_back(LkItem{(int)v, j0, j0 + c, -1});
             } else {
                 // at most 256 partial sums per run: one workgroup adds them
@@ -992,6 +1012,7 @@ extern "C" int tramp_lookup_create(tramp_ctx* ctx, int dtype, size_t n_rows, siz
         lk->tiles = (unsigned)tiles;
         lk->row = n_cols % piece ? LK_TAIL : n_cols * e % 128 ? LK_WHOLE : LK_LINES;
         lk->short_rows = short_rows;
+        lk->long_runs = long_runs;
         *out = lk;
         return TRAMP_OK;
     } catch (const std::exception&) {
@@ -1160,18 +1181,22 @@ static int launch_rows(tramp_ctx* ctx, const tramp_lookup* lk, size_t batch, con
         hipLaunchKernelGGL((lookup_chunks_kernel<T, ROW, MODE != LK_FWD && MODE != LK_MEAN>), dim3(lk->n_chunks * lk->tiles + (q ? 1 : 0), (unsigned)batch),
                            dim3(kBlock), 0, ctx->stream, a, q ? *q : LkScalArgs{}, x, w.partials);
     const dim3 grid = lk_grid(batch, blocks * lk->tiles, a.spread);
+    constexpr bool fwd = MODE == LK_FWD;
     if (MODE != LK_GRAD && self)
-        hipLaunchKernelGGL((lookup_rows_kernel<T, ROW, MODE, MODE != LK_GRAD>), grid, dim3(kBlock), 0, ctx->stream, a, *q, w.scal, bz, x, damping,
+        hipLaunchKernelGGL((lookup_rows_kernel<T, ROW, MODE, MODE != LK_GRAD, fwd>), grid, dim3(kBlock), 0, ctx->stream, a, *q, w.scal, bz, x, damping,
+                           b_old, out, r_out, w.partials, w.sr);
+    else if (blocks && fwd && lk->long_runs)
+        hipLaunchKernelGGL((lookup_rows_kernel<T, ROW, MODE, false, fwd>), grid, dim3(kBlock), 0, ctx->stream, a, LkScalArgs{}, w.scal, bz, x, damping,
                            b_old, out, r_out, w.partials, w.sr);
     else if (blocks)
-        hipLaunchKernelGGL((lookup_rows_kernel<T, ROW, MODE, false>), grid, dim3(kBlock), 0, ctx->stream, a, LkScalArgs{}, w.scal, bz, x, damping,
+        hipLaunchKernelGGL((lookup_rows_kernel<T, ROW, MODE, false, false>), grid, dim3(kBlock), 0, ctx->stream, a, LkScalArgs{}, w.scal, bz, x, damping,
                            b_old, out, r_out, w.partials, w.sr);
     if (a.n_lead) {
         LkArgs j = a;
         j.n_joins = j.blocks = lk->n_joins;
         j.n_lead = j.n_runs = j.n_waves = j.wave_blocks = j.n_light = j.light_blocks = j.n_single = j.single_blocks = j.n_empty = 0;
         j.spread = 0;
-        hipLaunchKernelGGL((lookup_rows_kernel<T, ROW, MODE, false>), lk_grid(batch, (size_t)j.blocks * lk->tiles, 0), dim3(kBlock), 0, ctx->stream,
+        hipLaunchKernelGGL((lookup_rows_kernel<T, ROW, MODE, false, false>), lk_grid(batch, (size_t)j.blocks * lk->tiles, 0), dim3(kBlock), 0, ctx->stream,
                            j, LkScalArgs{}, w.scal, bz, x, damping, b_old, out, r_out, w.partials, w.sr);
     }
     if (MODE == LK_FWD && lk->n_spreads)
