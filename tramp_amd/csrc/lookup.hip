@@ -42,7 +42,7 @@ struct tramp_lookup {
     const double* cnt;           // [2, K]  distinct counts and how many rows have them
     const LkItem* chunks;        // heavy runs in chunks, one partial sum each
     const LkItem* joins;         // {token, first chunk, one behind the last, index}
-    const LkItem* spreads;       // the chunks' positions and the padded ones
+    const LkItem* spreads;       // the chunks' positions
     const LkItem* runs;          // runs for one workgroup
     const LkItem* waves;         // runs for one wave
     const LkItem* light;         // the shorter runs, by falling length; slot: the first position
@@ -308,6 +308,7 @@ constexpr int kKeep = 8;
 constexpr int kEmpty = 4;
 // Rows that one position reads, two per group: gradient of 133588 x 76 f64 to 172932 rows 76.9 -> 70.8 us, the message to that table
 // 96.4 -> 84.9, to those positions 99.8 -> 77.6.  Four cost registers: 68.5, 92.9 and 77.0, but message to 8 x 10007 x 21 f64 46 -> 50.
+// Padded positions go with them (a launch of their own before: 31 x 152 f64 11.0 -> 8.1 us, 284412 x 9 f32, 30 % padded, 29.9 -> 23.5).
 constexpr int kOne = 2;
 
 struct LkArgs {
@@ -321,7 +322,8 @@ struct LkArgs {
     const int* empty;
     const int* idx;
     size_t V, D, T;
-    unsigned n_chunks, n_joins, n_runs, n_waves, wave_blocks, n_light, light_blocks, n_single, single_blocks, n_empty, n_multi, blocks, tiles, batch;
+    unsigned n_chunks, n_joins, n_runs, n_waves, wave_blocks, n_light, light_blocks, n_single, n_pad, single_blocks, n_empty, n_multi, blocks, tiles, batch;
+    size_t pad0;                 // the padded positions: perm[pad0 .. pad0 + n_pad), for the message to x
     unsigned n_lead;             // chunks summed in the launch of the runs (gradient)
     int lw, spread;
     double s;
@@ -555,27 +557,31 @@ __global__ __launch_bounds__(kBlock) void lookup_rows_kernel(LkArgs a, LkScalArg
             first = (threadIdx.x & 63) < (1u << a.lw);
         } else if ((MODE == LK_GRAD || MODE == LK_BWD || MODE == LK_FWD) && blk >= a.wave_blocks + a.light_blocks &&
                    blk < a.wave_blocks + a.light_blocks + a.single_blocks) {
-            // rows that one position reads, two per group
+            // rows that one position reads, two per group; behind them the padded positions (token -2), whose rx is 0
             const size_t G = kBlock >> a.lw, u0 = (size_t)(blk - a.wave_blocks - a.light_blocks) * kOne * G + k.group;
             LkItem it[kOne];
             T xs[kOne][N], zs[kOne][N];
             if (!act) return;
 #pragma unroll
-            for (int i = 0; i < kOne; ++i) it[i] = u0 + i * G < a.n_single ? a.light[a.n_light + u0 + i * G] : LkItem{-1, 0, 0, 0};
+            for (int i = 0; i < kOne; ++i) {
+                const size_t u = u0 + i * G;
+                it[i] = u < a.n_single ? a.light[a.n_light + u] : LkItem{-1, 0, 0, 0};
+                if (MODE == LK_FWD && u >= a.n_single && u - a.n_single < a.n_pad) it[i] = LkItem{-2, 0, 0, a.perm[a.pad0 + (u - a.n_single)]};
+            }
 #pragma unroll
             for (int i = 0; i < kOne; ++i)
-                if (it[i].token >= 0) {
+                if (it[i].token != -1) {
                     lk_load<T, ROW, true>(xb + (size_t)it[i].slot * a.D + k.col, k.valid, xs[i]);
-                    if (MODE != LK_GRAD) lk_load<T, ROW, MODE == LK_BWD>(bz + (b * a.V + (size_t)it[i].token) * a.D + k.col, k.valid, zs[i]);
+                    if (MODE != LK_GRAD && it[i].token >= 0) lk_load<T, ROW, MODE == LK_BWD>(bz + (b * a.V + (size_t)it[i].token) * a.D + k.col, k.valid, zs[i]);
                 }
             const double f = a.s / (c.az + c.lik1);
 #pragma unroll
             for (int i = 0; i < kOne; ++i) {
-                if (it[i].token < 0) continue;
+                if (it[i].token == -1) continue;
                 if (MODE == LK_FWD) {
                     double sr[N];
 #pragma unroll
-                    for (int e = 0; e < N; ++e) sr[e] = f * ((double)zs[i][e] + a.s * (0.0 + (double)xs[i][e]));
+                    for (int e = 0; e < N; ++e) sr[e] = it[i].token >= 0 ? f * ((double)zs[i][e] + a.s * (0.0 + (double)xs[i][e])) : 0.0;
                     lk_position_out<T, ROW>(a, c.ax + c.an, k, b, (size_t)it[i].slot, sr, xs[i], damping, b_old, out, r_out);
                 } else {
 #pragma unroll
@@ -713,9 +719,9 @@ __global__ __launch_bounds__(kBlock) void lookup_rows_kernel(LkArgs a, LkScalArg
         if (i < cnt) lk_position_out<T, ROW>(a, c.ax + c.an, k, b, (size_t)pj[i], sr, rows[i], damping, b_old, out, r_out);
 }
 
-// Third launch of the message to the positions: those of the heavy runs and the padded ones (slot -1: rx = 0), the chunks that were
-// summed last first - they are the likeliest to be cached still (10^6 x 64 f32: 150 us forwards, 138 us backwards).  Bound by
-// the write and what is read twice: 318 MB, 53 us, 6.0 TB/s.
+// Third launch of the message to the positions: those of the heavy runs, the chunks that were summed last first - they are the
+// likeliest to be cached still (10^6 x 64 f32: 150 us forwards, 138 us backwards).  Bound by the write and what is read twice:
+// 318 MB, 53 us, 6.0 TB/s.
 template <typename T, int ROW>
 __global__ __launch_bounds__(kBlock) void lookup_spread_kernel(LkArgs a, const LkItem* __restrict__ spreads, const LkScal* __restrict__ scal,
                                                                const double* __restrict__ sr_ws, const T* __restrict__ bx, double damping,
@@ -730,7 +736,7 @@ __global__ __launch_bounds__(kBlock) void lookup_spread_kernel(LkArgs a, const L
     double sr[N];
 #pragma unroll
     for (int e = 0; e < N; ++e)
-        sr[e] = it.slot >= 0 && e < k.valid ? sr_ws[(b * a.n_joins + (size_t)it.slot) * a.D + k.col + e] : 0.0;
+        sr[e] = e < k.valid ? sr_ws[(b * a.n_joins + (size_t)it.slot) * a.D + k.col + e] : 0.0;
     const int G = kBlock >> a.lw;
     for (int j = it.start + k.group; j < it.end; j += UR * G) {
         int t[UR];
@@ -918,8 +924,6 @@ extern "C" int tramp_lookup_create(tramp_ctx* ctx, int dtype, size_t n_rows, siz
                 joins.push_back(LkItem{(int)v, slot0, (int)chunks.size(), (int)joins.size()});
             }
         }
-        for (size_t j = seen; j < n_pos; j += (size_t)per_block)
-            spreads.push_back(LkItem{-1, (int)j, (int)std::min(n_pos, j + (size_t)per_block), -1});
         // equal lengths side by side: a wave goes no deeper than its longest run
         std::stable_sort(light.begin(), light.end(), [](const LkItem& x, const LkItem& y) { return x.end - x.start > y.end - y.start; });
         const size_t n_light2 = light.size();
@@ -1167,7 +1171,9 @@ static int launch_rows(tramp_ctx* ctx, const tramp_lookup* lk, size_t batch, con
     a.n_lead = MODE == LK_GRAD && lk->short_rows ? lk->n_chunks : 0;
     if (a.n_lead) a.n_joins = 0;
     a.light_blocks = (unsigned)(((size_t)a.n_light + G - 1) / G);
-    a.single_blocks = (unsigned)((a.n_single + kOne * G - 1) / (kOne * G));
+    a.n_pad = MODE == LK_FWD ? (unsigned)(lk->T - lk->seen) : 0;
+    a.pad0 = lk->seen;
+    a.single_blocks = (unsigned)(((size_t)a.n_single + a.n_pad + kOne * G - 1) / (kOne * G));
     const size_t blocks = (size_t)a.n_lead + a.n_joins + a.n_runs + a.wave_blocks + a.light_blocks + a.single_blocks + (a.n_empty + kEmpty * G - 1) / (kEmpty * G);
     TRAMP_REQUIRE(ctx, blocks * lk->tiles < 0x7fffffffu && (size_t)lk->n_spreads * lk->tiles < 0x7fffffffu &&
                            (size_t)lk->n_chunks * lk->tiles < 0x7ffffffeu);
@@ -1194,7 +1200,7 @@ static int launch_rows(tramp_ctx* ctx, const tramp_lookup* lk, size_t batch, con
     if (a.n_lead) {
         LkArgs j = a;
         j.n_joins = j.blocks = lk->n_joins;
-        j.n_lead = j.n_runs = j.n_waves = j.wave_blocks = j.n_light = j.light_blocks = j.n_single = j.single_blocks = j.n_empty = 0;
+        j.n_lead = j.n_runs = j.n_waves = j.wave_blocks = j.n_light = j.light_blocks = j.n_single = j.n_pad = j.single_blocks = j.n_empty = 0;
         j.spread = 0;
         hipLaunchKernelGGL((lookup_rows_kernel<T, ROW, MODE, false, false>), lk_grid(batch, (size_t)j.blocks * lk->tiles, 0), dim3(kBlock), 0, ctx->stream,
                            j, LkScalArgs{}, w.scal, bz, x, damping, b_old, out, r_out, w.partials, w.sr);
