@@ -355,6 +355,37 @@ def test_rows_that_few_positions_read(ctx, V, n, D, pad, dtype):
             assert (np.abs(damped[b] - want) <= eps2(dtype) * np.abs(want) + k * (mag + np.abs(b0[b]))).all()
 
 
+@pytest.mark.parametrize("dtype", [np.float64, np.float32])
+@pytest.mark.parametrize("V, n, D, heavy, pad", [(1, 1, 1, 0, 0), (40, 25, 5, 0, 0), (2000, 1201, 33, 0, 0), (30, 30, 260, 0, 0), (50, 41, 6, 3, 4),
+                                                 (700001, 600000, 1, 0, 0), (500000, 400000, 7, 2200, 0)])
+def test_a_position_alone_in_its_run_keeps_its_digits(ctx, V, n, D, heavy, pad, dtype):
+    """az far below ax scale^2: r (a + a') and b are both about b, the message is what bz has left.  Of a run of one it is
+    [s (ax + a') bz + (s^2 a' - az) bx] / prec, two terms that do not cancel: the kernel's a' is off by 2 (K + 8) u relative, a product or
+    quotient by u each, which 2 (K + 16) u of the terms' magnitudes holds.  The definition is taken in 64 bits of mantissa."""
+    import tramp_amd as T
+    rs = np.random.RandomState(V + n + D)
+    s = 0.7
+    tok = rs.permutation(V)[:n]
+    tok[:heavy], tok[n - pad:] = V - 1, -1
+    ch, ref = T.LookupChannel(tok, V, dim=D, scale=s, padding_index=-1, dtype=dtype, ctx=ctx), LookupFactor(tok, V, D, s)
+    az, ax = np.array([1.0, 0.3]), np.array([1e9, 3e6])
+    z = rs.standard_normal((2, V * D)).astype(dtype)
+    x = (ax[:, None] * rs.standard_normal((2, n * D))).astype(dtype)
+    a_d, b_d = ch.compute_forward_message(ctx.scalars(az), ctx.array(z, dtype), ctx.scalars(ax), ctx.array(x, dtype))
+    got = b_d.get().reshape(2, n, D)
+    K = np.unique(ref.count).size
+    one = np.flatnonzero((tok >= 0) & (ref.count[np.maximum(tok, 0)] == 1))
+    L = np.longdouble
+    for b in range(2):
+        ra = ref._a(ref.forward_variance(az[b], ax[b]), ax[b])
+        zz, xx = z[b].reshape(V, D)[tok[one]].astype(L), x[b].reshape(n, D)[one].astype(L)
+        prec = L(az[b]) + L(ax[b]) * L(s) * L(s)
+        kz, kx = L(s) * (L(ax[b]) + L(ra)) / prec, (L(s) * L(s) * L(ra) - L(az[b])) / prec
+        want = kz * zz + kx * xx
+        mag = np.abs(kz * zz) + np.abs(xx) * (L(s) * L(s) * L(ra) + L(az[b])) / prec
+        assert (np.abs(got[b, one] - want) <= eps2(dtype) * np.abs(want) + 2 * (K + 16) * U * mag).all(), b
+
+
 def test_a_precision_that_is_nan_stays_one(ctx):
     import tramp_amd as T
     ch = T.LookupChannel([0, 1, 1], 3, ctx=ctx)

@@ -7,11 +7,12 @@
 //     r_v  = (bz_v + g_v) / prec_v                                  posterior mean of the table
 //     rx_t = scale r_{token_t}                                      posterior mean of the positions (0 where padded)
 //     vz   = (1/V) sum_v 1 / prec_v            vx = (scale^2 / T) sum_v count_v / prec_v
-// and the messages a' = clip(1/v - a), b' = r (a + a') - b (tramp/base.py:250-255).  Both ends of 1/v - a and of the b' to
-// the table are sums without cancellation, which is how they are formed here:
+// and the messages a' = clip(1/v - a), b' = r (a + a') - b (tramp/base.py:250-255).  Both ends of 1/v - a, the b' to the table and
+// the b' to a position that reads its row alone are sums without cancellation, which is how they are formed here:
 //     1/vz - az = [(1/V) sum_v lik_v / prec_v] / vz
 //     1/vx - ax = [padded / T + (1/T) sum_v count_v (az + ax scale^2 (count_v - 1)) / prec_v] / vx
 //     b'_v = [g_v (az + a') + bz_v (a' - lik_v)] / prec_v
+//     b'_t = [s (ax + a') bz_v + (s^2 a' - az) bx_t] / prec_v       where t is the only position of v; otherwise rx_t (ax + a') - bx_t
 // (a table of 10^5 rows of which ten are read has a' of order 10^-4 az: the difference would lose the digits of f64).
 //
 // The positions are sorted by token once, at creation (perm, off): the adjoint is a sum over runs, in a fixed order, without
@@ -416,27 +417,46 @@ __device__ __forceinline__ void lk_row_out(const LkArgs& a, const LkScal& c, con
     lk_store<T, ROW>(out + at, k.valid, o);
 }
 
-// the message to one position: b' = rx (ax + a') - bx with rx = scale r
+// the message m to one position, and rx = scale r
 template <typename T, int ROW>
-__device__ __forceinline__ void lk_position_out(const LkArgs& a, double asum, const LkLane& k, size_t b, size_t t,
-                                                const double (&sr)[LkVec<T>::N], const T (&bx)[LkVec<T>::N], double damping, const T* b_old,
-                                                T* out, T* __restrict__ r_out) {
+__device__ __forceinline__ void lk_position_store(const LkArgs& a, const LkLane& k, size_t b, size_t t, const double (&m)[LkVec<T>::N],
+                                                  const double (&sr)[LkVec<T>::N], double damping, const T* b_old, T* out,
+                                                  T* __restrict__ r_out) {
     constexpr int N = LkVec<T>::N;
     const size_t at = (b * a.T + t) * a.D + k.col;
     T o[N], old[N];
     if (damping != 0.0) lk_load<T, ROW>(b_old + at, k.valid, old);
 #pragma unroll
-    for (int e = 0; e < N; ++e) {
-        double m = sr[e] * asum - (double)bx[e];
-        if (damping != 0.0) m = damping * (double)old[e] + (1.0 - damping) * m;
-        o[e] = T(m);
-    }
+    for (int e = 0; e < N; ++e) o[e] = T(damping != 0.0 ? damping * (double)old[e] + (1.0 - damping) * m[e] : m[e]);
     lk_store<T, ROW>(out + at, k.valid, o);
     if (r_out) {
 #pragma unroll
         for (int e = 0; e < N; ++e) o[e] = T(sr[e]);
         lk_store<T, ROW>(r_out + at, k.valid, o);
     }
+}
+
+// b' = rx (ax + a') - bx
+template <typename T, int ROW>
+__device__ __forceinline__ void lk_position_out(const LkArgs& a, double asum, const LkLane& k, size_t b, size_t t,
+                                                const double (&sr)[LkVec<T>::N], const T (&bx)[LkVec<T>::N], double damping, const T* b_old,
+                                                T* out, T* __restrict__ r_out) {
+    constexpr int N = LkVec<T>::N;
+    double m[N];
+#pragma unroll
+    for (int e = 0; e < N; ++e) m[e] = sr[e] * asum - (double)bx[e];
+    lk_position_store<T, ROW>(a, k, b, t, m, sr, damping, b_old, out, r_out);
+}
+
+// A position alone in its run: b' = kz bz + kx bx.  Where ax s^2 is far above az, rx (ax + a') and bx agree in most of their digits
+// (a' is about az / s^2) and the difference would be left with none of bz's; kz bz and kx bx do not cancel.  A longer run says
+// itself what bx does not: its difference is off by roundings of bx, as that of the definition.
+struct LkOne {
+    double mean, kz, kx;             // rx = mean (bz + s bx)
+};
+__device__ __forceinline__ LkOne lk_one(const LkScal& c, double s) {
+    const double inv = 1.0 / (c.az + c.lik1), mean = s * inv;
+    return LkOne{mean, mean * (c.ax + c.an), fma(s * s, c.an, -c.az) * inv};
 }
 
 // the partial sum of a chunk of a heavy run
@@ -574,15 +594,19 @@ __global__ __launch_bounds__(kBlock) void lookup_rows_kernel(LkArgs a, LkScalArg
                     lk_load<T, ROW, true>(xb + (size_t)it[i].slot * a.D + k.col, k.valid, xs[i]);
                     if (MODE != LK_GRAD && it[i].token >= 0) lk_load<T, ROW, MODE == LK_BWD>(bz + (b * a.V + (size_t)it[i].token) * a.D + k.col, k.valid, zs[i]);
                 }
-            const double f = a.s / (c.az + c.lik1);
+            const LkOne one = lk_one(c, a.s);
 #pragma unroll
             for (int i = 0; i < kOne; ++i) {
                 if (it[i].token == -1) continue;
                 if (MODE == LK_FWD) {
-                    double sr[N];
+                    double sr[N], m[N];
 #pragma unroll
-                    for (int e = 0; e < N; ++e) sr[e] = it[i].token >= 0 ? f * ((double)zs[i][e] + a.s * (0.0 + (double)xs[i][e])) : 0.0;
-                    lk_position_out<T, ROW>(a, c.ax + c.an, k, b, (size_t)it[i].slot, sr, xs[i], damping, b_old, out, r_out);
+                    for (int e = 0; e < N; ++e) {
+                        const double bz_e = (double)zs[i][e], bx_e = (double)xs[i][e];
+                        sr[e] = it[i].token >= 0 ? one.mean * (bz_e + a.s * bx_e) : 0.0;
+                        m[e] = it[i].token >= 0 ? one.kz * bz_e + one.kx * bx_e : 0.0 * (c.ax + c.an) - bx_e;
+                    }
+                    lk_position_store<T, ROW>(a, k, b, (size_t)it[i].slot, m, sr, damping, b_old, out, r_out);
                 } else {
 #pragma unroll
                     for (int e = 0; e < N; ++e) acc[e] = 0.0 + (double)xs[i][e];
@@ -770,7 +794,8 @@ __global__ __launch_bounds__(kBlock) void lookup_positions_kernel(LkArgs a, cons
     const LkLane k = lk_lane<T>(a.lw, place.tile, a.D);
     if (!place.in || k.valid <= 0) return;
     const LkScal c = scal[b];
-    const double asum = c.ax + c.an, f1 = a.s / (c.az + c.lik1);
+    const double asum = c.ax + c.an;
+    const LkOne one = lk_one(c, a.s);
     const size_t G = kBlock >> a.lw, t0 = (size_t)place.blk * UR * G + k.group;
     int w[UR];
     T v[UR][N], z[UR][N];
@@ -787,11 +812,14 @@ __global__ __launch_bounds__(kBlock) void lookup_positions_kernel(LkArgs a, cons
     }
 #pragma unroll
     for (int i = 0; i < UR; ++i) {
-        if (w[i] <= -2) {
+        double m[N];
 #pragma unroll
-            for (int e = 0; e < N; ++e) sr[i][e] = f1 * ((double)z[i][e] + a.s * (double)v[i][e]);
+        for (int e = 0; e < N; ++e) {
+            const double bx_e = (double)v[i][e], bz_e = (double)z[i][e];
+            if (w[i] <= -2) sr[i][e] = one.mean * (bz_e + a.s * bx_e);
+            m[e] = w[i] <= -2 ? one.kz * bz_e + one.kx * bx_e : sr[i][e] * asum - bx_e;
         }
-        if (t0 + i * G < a.T) lk_position_out<T, ROW>(a, asum, k, b, t0 + i * G, sr[i], v[i], damping, b_old, out, r_out);
+        if (t0 + i * G < a.T) lk_position_store<T, ROW>(a, k, b, t0 + i * G, m, sr[i], damping, b_old, out, r_out);
     }
 }
 
@@ -805,7 +833,8 @@ __global__ __launch_bounds__(kBlock) void lookup_positions1_kernel(LkArgs a, con
     const size_t b = place.b, t = ((size_t)place.blk * kBlock + threadIdx.x) * N;
     if (!place.in || t >= a.T) return;
     const LkScal c = scal[b];
-    const double asum = c.ax + c.an, f1 = a.s / (c.az + c.lik1);
+    const double asum = c.ax + c.an;
+    const LkOne one = lk_one(c, a.s);
     const int valid = a.T - t >= N ? N : (int)(a.T - t);
     int w[N];
     T v[N], o[N], old[N];
@@ -829,8 +858,8 @@ __global__ __launch_bounds__(kBlock) void lookup_positions1_kernel(LkArgs a, con
         z[i] = w[i] >= 0 ? sr_ws[b * a.n_multi + (size_t)w[i]] : w[i] == -1 ? 0.0 : (double)bz[b * a.V + (size_t)(-2 - w[i])];
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-        if (w[i] <= -2) z[i] = f1 * (z[i] + a.s * (double)v[i]);
-        double m = z[i] * asum - (double)v[i];
+        double m = w[i] <= -2 ? one.kz * z[i] + one.kx * (double)v[i] : z[i] * asum - (double)v[i];
+        if (w[i] <= -2) z[i] = one.mean * (z[i] + a.s * (double)v[i]);
         if (damping != 0.0) m = damping * (double)old[i] + (1.0 - damping) * m;
         o[i] = T(m);
     }
