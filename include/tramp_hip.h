@@ -597,8 +597,8 @@ int tramp_group_clip(tramp_ctx* ctx, const tramp_group* group, double max_norm, 
 /* out = prev + min(1, max_step / |x_b - prev_b|) (x - prev), the step of a set of messages bounded like constant damping with a
  * factor per instance (tramp/algos/message_passing.py:119-127).  a_d, a_prev_d [n_a, batch] (optional): precisions that move
  * by the same factor, in place in a_d.  refresh != 0: the result is written over prev (and a_prev) as well.  An instance whose
- * step is not finite takes it whole, for the NaN guard to see.  norm_d, a_d and a_prev_d touch neither each other nor an array
- * of the lists (checked). */
+ * step is not finite takes it whole, for the NaN guard to see, and so does a precision whose own step is not.  norm_d, a_d and
+ * a_prev_d touch neither each other nor an array of the lists (checked). */
 int tramp_group_limit_step(tramp_ctx* ctx, const tramp_group* group, const tramp_group* prev, double max_step,
                            const tramp_group* out, int refresh, size_t n_a, double* a_d, double* a_prev_d, double* norm_d);
 

@@ -208,6 +208,19 @@ def test_precisions_that_are_infinite_stay_so(ctx):
         assert a.get()[:, 0] == pytest.approx([np.inf, 3.0, np.inf], rel=1e-14)
 
 
+@pytest.mark.parametrize("n", [3, 50000])                              # one launch, two launches
+@pytest.mark.parametrize("refresh", [False, True])
+def test_precisions_whose_step_is_not_finite_take_it_whole(ctx, n, refresh):
+    import tramp_amd as T
+    x, p = T.ArrayGroup([ctx.array(np.full((1, n), 2.0))]), T.ArrayGroup([ctx.zeros((1, n), np.float64)])
+    new, old = np.array([[4.0], [np.inf], [3.0], [np.nan], [-1e308], [5.0]]), np.array([[np.inf], [4.0], [np.nan], [2.0], [1e308], [1.0]])
+    a, a_prev = ctx.array(new), ctx.array(old)
+    norm = x.limit_step(p, np.sqrt(n), a=a, a_prev=a_prev, refresh=refresh).get()      # factor 1/2
+    assert norm[0] == pytest.approx(2 * np.sqrt(n), rel=1e-14)
+    assert np.array_equal(a.get()[:5], new[:5], equal_nan=True) and a.get()[5, 0] == pytest.approx(3.0, rel=1e-14)
+    assert np.array_equal(a_prev.get(), a.get() if refresh else old, equal_nan=True)
+
+
 def test_replays_equal_the_eager_calls(ctx):
     import tramp_amd as T
     rs = np.random.RandomState(9)

@@ -185,8 +185,8 @@ template <bool STEP> __device__ __forceinline__ void group_side(const GroupSide&
     if (threadIdx.x == 0 && q.norm_out) q.norm_out[b] = norm;
     if (!STEP) return;
     for (size_t i = threadIdx.x; i < q.n_a; i += kBlock) {
-        const double o = q.a_prev[i * q.batch + b], x = q.a[i * q.batch + b];
-        const double r = c < 1.0 && x != o ? o + c * (x - o) : x;          // infinite before and after: so it stays
+        const double o = q.a_prev[i * q.batch + b], x = q.a[i * q.batch + b], d = x - o;
+        const double r = c < 1.0 && d - d == 0.0 ? o + c * d : x;          // a step that is infinite or NaN is taken whole
         q.a[i * q.batch + b] = r;
         if (q.refresh) q.a_prev[i * q.batch + b] = r;
     }
