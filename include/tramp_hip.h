@@ -572,11 +572,13 @@ int tramp_lookup_destroy(tramp_ctx* ctx, tramp_lookup* lookup);
 int tramp_lookup_apply(tramp_ctx* ctx, tramp_lookup* lookup, size_t batch, const void* z_d, void* x_d);
 /* The adjoint: g[b, v, :] = scale sum of x[b, t, :] over the positions t of token v (0 for a token without positions). */
 int tramp_lookup_gradient(tramp_ctx* ctx, tramp_lookup* lookup, size_t batch, const void* x_d, void* g_d);
-/* LinearChannel.compute_n_eff / compute_*_variance (linear_channel.py:58-67, 91-105); v_d, a_new_d, n_eff_d optional. */
+/* LinearChannel.compute_n_eff / compute_*_variance (linear_channel.py:58-67, 91-105); v_d, a_new_d, n_eff_d optional, each apart
+ * from the others and either apart from az_d and ax_d or exactly one of them (checked). */
 int tramp_lookup_variance(tramp_ctx* ctx, tramp_lookup* lookup, int dir, size_t batch, const double* az_d, const double* ax_d,
                           double* v_d, double* a_new_d, double* n_eff_d);
 /* dir BWD: the message to z ([batch, n_rows, n_cols]), FWD: to x ([batch, n_pos, n_cols]); r_d, v_d optional posterior.
- * b_new_d and r_d must not overlap bz_d, bx_d or each other, nor r_d b_old_d; a_old_d / b_old_d may be a_new_d / b_new_d. */
+ * Results must not overlap each other or what is read (checked), but for exact identity: a_new_d and v_d may be az_d, ax_d or
+ * a_old_d, b_new_d may be b_old_d. */
 int tramp_lookup_message(tramp_ctx* ctx, tramp_lookup* lookup, int dir, size_t batch, const double* az_d, const void* bz_d,
                          const double* ax_d, const void* bx_d, double damping, const double* a_old_d, const void* b_old_d,
                          double* a_new_d, void* b_new_d, void* r_d, double* v_d);

@@ -477,6 +477,42 @@ def test_refusals_on_the_device(ctx):
         other.close()
 
 
+@pytest.mark.parametrize("V, n, D, B", [(20, 30, 3, 4), (9, 5, 1, 2), (3, 9000, 2, 3), (400, 70000, 4, 3)])
+def test_scalar_results_in_place_and_shifted(ctx, V, n, D, B):
+    "a' or v over the precisions it is made of: the bits of the call with buffers of its own, in every form; shifted: refused"
+    import tramp_amd as T
+    rs = np.random.RandomState(n)
+    ch = T.LookupChannel(zipf_tokens(rs, V, n, 0.6, 0.1), V, dim=D, padding_index=-1, ctx=ctx)
+    z, x = ctx.array(rs.standard_normal((B, V * D))), ctx.array(rs.standard_normal((B, n * D)))
+    scal = {"az": rs.uniform(0.5, 2, B), "ax": rs.uniform(0.1, 3, B), "a_old": rs.uniform(0.5, 2, B)}
+    for direction, m in ((T._lib.FWD, n * D), (T._lib.BWD, V * D)):
+        old = ctx.array(rs.standard_normal((B, m)))
+
+        def run(a_new=None, v=None, shift=0):
+            d = {k: ctx.array(np.concatenate([s, np.zeros(1)])) for k, s in scal.items()}
+            put = lambda name: d[name].ptr + 8 * shift if name else d.setdefault("own" + str(len(d)), ctx.empty((B,))).ptr      # noqa: E731
+            pa, pv, b, r = put(a_new), put(v), ctx.empty((B, m)), ctx.empty((B, m))
+            ctx._call("tramp_lookup_message", ch._handle, direction, B, d["az"].ptr, z.ptr, d["ax"].ptr, x.ptr, 0.25, d["a_old"].ptr, old.ptr,
+                      pa, b.ptr, r.ptr, pv)
+            return [T.DeviceArray(ctx, (B,), np.float64, ptr=q, owner=False).get() for q in (pa, pv)] + [b.get(), r.get()]
+        want = run()
+        for over in (dict(a_new="az"), dict(a_new="ax"), dict(v="az"), dict(v="ax"), dict(v="a_old"), dict(a_new="ax", v="az")):
+            for got, w in zip(run(**over), want):
+                assert np.array_equal(got, w), over
+            with pytest.raises(T._lib.TrampHipError):
+                run(**over, shift=1)
+    both = ctx.array(np.arange(1.0, 2 * B + 1))
+    at = lambda i: both.ptr + 8 * i                                    # noqa: E731
+    for args in ((at(0), at(B), at(1), None, None), (at(0), at(B), None, at(B - 1), None), (at(0), at(0), at(B), at(B), None),
+                 (at(0), at(0), None, at(B), at(B - 1))):
+        with pytest.raises(T._lib.TrampHipError):
+            ctx._call("tramp_lookup_variance", ch._handle, T._lib.FWD, B, *args)
+    assert np.array_equal(both.get(), np.arange(1.0, 2 * B + 1))
+    out = ctx.empty((B, n * D))
+    with pytest.raises(T._lib.TrampHipError):                         # a vector over the precisions
+        ctx._call("tramp_lookup_message", ch._handle, T._lib.FWD, B, out.ptr + 8, z.ptr, at(0), x.ptr, 0.0, None, None, at(B), out.ptr, None, None)
+
+
 # ---------------------------------------------------------------- in models
 def regression(T, ctx, channel, V, y, prior="gb"):
     pri = T.GaussBernoulliPrior(size=V, rho=0.5, ctx=ctx)

@@ -1,6 +1,8 @@
 """Refusals of the lookup channel, of the array lists and of iterate(max_step=...) that need no device, and the plain
 definitions the GPU tests compare with, checked against the dense oracle of the linear channel."""
 import ctypes as C
+import os
+import subprocess
 
 import numpy as np
 import pytest
@@ -140,6 +142,53 @@ def test_c_entries_refuse_a_null_context():
     assert lib.tramp_group_clip(None, None, 1.0, None, None) == T._lib.EINVAL
     assert lib.tramp_group_limit_step(None, None, None, 1.0, None, 0, 0, None, None, None) == T._lib.EINVAL
     assert lib.tramp_group_destroy(None, None) == T._lib.EINVAL
+
+
+@pytest.fixture(scope="module")
+def buffers(tmp_path_factory):
+    "csrc/lookup_buffers.h behind two C functions"
+    d = tmp_path_factory.mktemp("buffers")
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    (d / "b.cpp").write_text('#include <initializer_list>\n#include "lookup_buffers.h"\n'
+                             'extern "C" const char* conflict(const LkBuffers* m) { return lk_conflict(*m); }\n'
+                             'extern "C" int in_place(const void* az, const void* ax, const void* a, const void* v, const void* n) '
+                             '{ return lk_scalars_in_place(az, ax, a, v, n); }\n')
+    subprocess.run(["g++", "-std=c++17", "-Wall", "-Werror", "-shared", "-fPIC", "-I", os.path.join(root, "tramp_amd", "csrc"), str(d / "b.cpp"),
+                    "-o", str(d / "b.so")], check=True)
+    lib = C.CDLL(str(d / "b.so"))
+    lib.conflict.restype = C.c_char_p
+    lib.in_place.argtypes = [C.c_void_p] * 5
+    return lib
+
+
+# 2 instances, z of 2 x 3 doubles, x of 2 x 5, message to x; every buffer on a page of its own
+PLACES = dict(az=0x1000, ax=0x2000, a_old=0x3000, bz=0x4000, bx=0x5000, b_old=0x6000, a_new=0x7000, v=0x8000, n_eff=0, b_new=0x9000, r=0xa000)
+SIZES = dict(scal=16, nz=48, nx=80, nout=80)
+
+
+@pytest.mark.parametrize("moved, fine", [
+    ({}, True), (dict(a_new=0x3000, b_new=0x6000), True), (dict(a_new=0x1000), True), (dict(v=0x1000), True), (dict(v=0x2000), True),
+    (dict(v=0x3000), True), (dict(a_new=0x1000, v=0x2000), True), (dict(a_new=0x1010), True), (dict(r=0), True), (dict(a_new=0x5050), True),
+    (dict(a_new=0x1008), False), (dict(a_new=0xff8), False), (dict(v=0x2008), False), (dict(v=0x3008), False), (dict(v=0x7000), False),
+    (dict(v=0x7008), False), (dict(a_new=0x4000), False), (dict(a_new=0x5048), False), (dict(v=0x6040), False), (dict(v=0x9000), False),
+    (dict(a_new=0xa040), False), (dict(b_new=0x1000), False), (dict(b_new=0x2008), False), (dict(r=0x2000 - 72), False), (dict(r=0x3000), False),
+    (dict(b_new=0x5000), False), (dict(b_new=0x4028), False), (dict(b_new=0x6008), False), (dict(r=0x6000), False), (dict(r=0x9008), False),
+    (dict(n_eff=0x7008), False), (dict(n_eff=0x1000), True), (dict(n_eff=0x1008), False)])
+def test_results_over_what_is_read(buffers, moved, fine):
+    fields = ["az", "ax", "a_old", "bz", "bx", "b_old", "a_new", "v", "n_eff", "b_new", "r"]
+
+    class Buffers(C.Structure):
+        _fields_ = [(f, C.c_void_p) for f in fields] + [(f, C.c_size_t) for f in ("scal", "nz", "nx", "nout")]
+    got = buffers.conflict(C.byref(Buffers(**{**PLACES, **SIZES, **moved})))
+    assert (got is None) == fine, got
+
+
+def test_scalars_over_the_precisions_are_seen(buffers):
+    a, b, c, d, e = 0x1000, 0x2000, 0x3000, 0x4000, 0x5000
+    assert not buffers.in_place(a, b, c, d, e) and not buffers.in_place(a, b, None, None, None)
+    for over in (a, b):
+        for results in ((over, d, e), (c, over, e), (c, d, over)):
+            assert buffers.in_place(a, b, *results)
 
 
 def test_iterate_refuses_bad_steps():

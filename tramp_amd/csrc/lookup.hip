@@ -19,6 +19,7 @@
 // atomics, the same bits every time.  All arithmetic is in double and rounded once to the element type at the store: the
 // passes are bound by memory (a few operations per element), the conversions are free next to the loads.
 #include "common.h"
+#include "lookup_buffers.h"
 #include "tramp_math.h"
 
 #include <algorithm>
@@ -120,9 +121,10 @@ __device__ __forceinline__ LkScal lk_scalars(const LkScalArgs& q, size_t b, bool
     const LkScal c{az, ax, an, lik1};
     if (write && threadIdx.x == 0) {
         if (q.scal) q.scal[b] = c;
+        // a' before v: v may replace a_old, whose scalar load is only waited for where its value is used
+        if (q.a_new_out) q.a_new_out[b] = q.damping != 0.0 ? q.damping * q.a_old[b] + (1.0 - q.damping) * an : an;
         if (q.v_out) q.v_out[b] = v;
         if (q.n_eff_out) q.n_eff_out[b] = se / q.V;
-        if (q.a_new_out) q.a_new_out[b] = q.damping != 0.0 ? q.damping * q.a_old[b] + (1.0 - q.damping) * an : an;
     }
     return c;
 }
@@ -1066,12 +1068,6 @@ extern "C" int tramp_lookup_destroy(tramp_ctx* ctx, tramp_lookup* lk) {
     TRAMP_REQUIRE(ctx, lk && lk->device == ctx->device);     \
     TRAMP_REQUIRE(ctx, batch <= 65535)
 
-// do the rows of x and y (bytes each) share memory?
-static bool lk_overlap(const void* x, size_t nx, const void* y, size_t ny) {
-    const uintptr_t a = (uintptr_t)x, b = (uintptr_t)y;
-    return x && y && a < b + ny && b < a + nx;
-}
-
 // CALL(ROW) for the handle's kind of rows
 #define LK_BY_ROW(lk, CALL)               \
     switch ((lk)->row) {                  \
@@ -1210,8 +1206,8 @@ static int launch_rows(tramp_ctx* ctx, const tramp_lookup* lk, size_t batch, con
     a.spread = lk_spread(batch, blocks * lk->tiles, lk->T * lk->D * sizeof(T), 2u << 20);
     // few workgroups and few counts: each makes the scalars for itself, one launch less (V = 1000, 2000 positions 10.2 -> 7.6 us;
     // with up to 4096 workgroups 8 x 60000 x 8 f64 would be 31.5 against 27.1 us)
-    const bool self = q && !lk->n_chunks && blocks && blocks * lk->tiles * batch <= 1024 && lk->K <= 4 * kBlock && q->a_new_out != q->az &&
-                      q->a_new_out != q->ax;
+    const bool self = q && !lk->n_chunks && blocks && blocks * lk->tiles * batch <= 1024 && lk->K <= 4 * kBlock &&
+                      !lk_scalars_in_place(q->az, q->ax, q->a_new_out, q->v_out, q->n_eff_out);
     if ((lk->n_chunks && !a.n_lead) || (q && !self))
         hipLaunchKernelGGL((lookup_chunks_kernel<T, ROW, MODE != LK_FWD && MODE != LK_MEAN>), dim3(lk->n_chunks * lk->tiles + (q ? 1 : 0), (unsigned)batch),
                            dim3(kBlock), 0, ctx->stream, a, q ? *q : LkScalArgs{}, x, w.partials);
@@ -1278,6 +1274,9 @@ extern "C" int tramp_lookup_variance(tramp_ctx* ctx, tramp_lookup* lk, int dir, 
                                      const double* ax_d, double* v_d, double* a_new_d, double* n_eff_d) {
     LK_REQUIRE_CALL(ctx, lk, batch);
     TRAMP_REQUIRE(ctx, (dir == TRAMP_FWD || dir == TRAMP_BWD) && az_d && ax_d);
+    const char* conflict = lk_conflict({az_d, ax_d, nullptr, nullptr, nullptr, nullptr, a_new_d, v_d, n_eff_d, nullptr, nullptr, batch * sizeof(double),
+                                        0, 0, 0});
+    if (conflict) return tramp_fail(ctx, TRAMP_EINVAL, "tramp_lookup_variance", conflict);
     if (!batch) return TRAMP_OK;
     LkScalArgs q = lk_scal_args(lk, dir, az_d, ax_d, 0.0, nullptr);
     q.v_out = v_d;
@@ -1311,12 +1310,11 @@ extern "C" int tramp_lookup_message(tramp_ctx* ctx, tramp_lookup* lk, int dir, s
     LK_REQUIRE_CALL(ctx, lk, batch);
     TRAMP_REQUIRE(ctx, (dir == TRAMP_FWD || dir == TRAMP_BWD) && az_d && bz_d && ax_d && bx_d && a_new_d && b_new_d);
     const size_t row = batch * lk->D * dtype_size(lk->dtype), nz = lk->V * row, nx = lk->T * row, no = dir == TRAMP_FWD ? nx : nz;
-    TRAMP_REQUIRE(ctx, !lk_overlap(b_new_d, no, bz_d, nz) && !lk_overlap(b_new_d, no, bx_d, nx));
-    TRAMP_REQUIRE(ctx, !lk_overlap(r_d, no, bz_d, nz) && !lk_overlap(r_d, no, bx_d, nx) && !lk_overlap(r_d, no, b_new_d, no));
-    TRAMP_REQUIRE(ctx, damping == 0.0 || b_old_d == b_new_d || !lk_overlap(b_old_d, no, b_new_d, no));
-    TRAMP_REQUIRE(ctx, damping == 0.0 || !lk_overlap(b_old_d, no, r_d, no));
-    TRAMP_REQUIRE(ctx, damping == 0.0 || !lk_overlap(b_old_d, no, r_d, no));
     TRAMP_REQUIRE(ctx, damping == 0.0 || (a_old_d && b_old_d));
+    const bool damped = damping != 0.0;
+    const char* conflict = lk_conflict({az_d, ax_d, damped ? a_old_d : nullptr, bz_d, bx_d, damped ? b_old_d : nullptr, a_new_d, v_d, nullptr, b_new_d, r_d,
+                                        batch * sizeof(double), nz, nx, no});
+    if (conflict) return tramp_fail(ctx, TRAMP_EINVAL, "tramp_lookup_message", conflict);
     if (!batch) return TRAMP_OK;
     if (lk->dtype == TRAMP_F64)
         return lookup_message<double>(ctx, lk, dir, batch, az_d, (const double*)bz_d, ax_d, (const double*)bx_d, damping, a_old_d,
