@@ -2,6 +2,7 @@
 #include "common.h"
 #include "linear.h"
 #include "prior_hint.h"
+#include "workspace.h"
 #include <stdlib.h>
 
 static void flush_deferred_frees(tramp_ctx* ctx);
@@ -42,7 +43,7 @@ extern "C" int tramp_ctx_create(int device, tramp_ctx** out) {
     }
     hipDeviceProp_t prop;
     if (hipGetDeviceProperties(&prop, device) == hipSuccess) ctx->num_cu = prop.multiProcessorCount;
-    ctx->ws_bytes = 4u << 20;
+    ctx->ws_bytes = kWsFirst;
     if (hipMalloc((void**)&ctx->ws, ctx->ws_bytes) != hipSuccess) {
         (void)hipStreamDestroy(ctx->stream);
         delete ctx;
@@ -219,17 +220,17 @@ int tramp_ws_reserve(tramp_ctx* ctx, size_t bytes) {
                           "workspace, which this call would have to re-allocate; destroy the graph first or use "
                           "another context for the larger call");
     (void)hipSetDevice(ctx->device);
-    size_t nb = ctx->ws_bytes;
-    while (nb < bytes) nb *= 2;
     TRAMP_HIP_CHECK(ctx, hipStreamSynchronize(ctx->stream));
-    TRAMP_HIP_CHECK(ctx, hipFree(ctx->ws));
-    ctx->ws = nullptr;
-    ctx->ws_bytes = 0;
-    if (hipMalloc((void**)&ctx->ws, nb) != hipSuccess) {
+    const auto alloc = [](size_t n) -> void* {
+        void* p = nullptr;
+        if (hipMalloc(&p, n) == hipSuccess) return p;
         (void)hipGetLastError();
-        return tramp_fail(ctx, TRAMP_ENOMEM, "workspace", "hipMalloc failed");
-    }
-    ctx->ws_bytes = nb;
+        return nullptr;
+    };
+    void* ws = ctx->ws;
+    const bool grown = ws_grow(&ws, &ctx->ws_bytes, bytes, alloc, [](void* p) { (void)hipFree(p); });
+    ctx->ws = static_cast<double*>(ws);
+    if (!grown) return tramp_fail(ctx, TRAMP_ENOMEM, "workspace", "hipMalloc failed");
     return TRAMP_OK;
 }
 
