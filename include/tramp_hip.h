@@ -563,7 +563,8 @@ int tramp_conv_message(tramp_ctx* ctx, tramp_conv* conv, int dir, size_t batch,
  * with one entry `scale` per row, for z = [batch, n_rows, n_cols] and x = [batch, n_pos, n_cols].  tokens_h (host): [n_pos],
  * the row each position reads, -1 for a padded position (a zero row of W: x = 0 there).  The positions are sorted by token
  * once, here; W^T W = scale^2 diag(count) makes variances, messages and log-partition closed forms (csrc/lookup.hip).
- * n_rows, n_cols, n_pos <= 2^31 - 2^16; sums over positions are in double, in a fixed order, without atomics. */
+ * n_rows, n_cols, n_pos <= 2^31 - 2^16; sums over positions are in double, in a fixed order, without atomics.  A call that
+ * would take 2^24 workgroups or more per instance (vectors of more than 2^30 rows or some 60 GB) is refused. */
 typedef struct tramp_lookup tramp_lookup;
 int tramp_lookup_create(tramp_ctx* ctx, int dtype, size_t n_rows, size_t n_cols, size_t n_pos, const int* tokens_h,
                         double scale, tramp_lookup** lookup);

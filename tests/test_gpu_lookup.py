@@ -424,6 +424,22 @@ def test_offsets_beyond_32_bits(ctx):
     assert np.array_equal(row(b, n - 1), np.zeros(D, np.float32)) and a.get()[0] == pytest.approx(ra, rel=1e-12)
 
 
+def test_more_instances_than_one_axis_of_a_grid_holds(ctx):
+    "65528 instances of 65700 rows: 1.68e7 workgroups of 256; every component of the 17 GB is written, one per instance not zero"
+    import tramp_amd as T
+    B, V = 65528, 65700
+    ch = T.LookupChannel([V - 3], V, scale=2.0, dtype=np.float32, ctx=ctx)
+    x = np.arange(1, B + 1, dtype=np.float32)[:, None]
+    g = ctx.full((B, V), np.nan, np.float32)
+    ch.gradient(ctx.array(x, np.float32), out=g)
+    assert np.array_equal(T.ArrayGroup([g]).norm().get(), 2.0 * x[:, 0])
+    for b in (0, 1, B // 2, B - 1):
+        row = T.DeviceArray(ctx, (V,), np.float32, ptr=g.ptr + 4 * b * V, owner=False).get()
+        assert row[V - 3] == 2.0 * x[b, 0] and np.count_nonzero(row) == 1
+    X = ch.lookup(g).get()
+    assert np.array_equal(X, 4.0 * x)
+
+
 def test_refusals_on_the_device(ctx):
     import tramp_amd as T
     ch = T.LookupChannel([0, 1, 1], 2, ctx=ctx)

@@ -191,6 +191,22 @@ def test_scalars_over_the_precisions_are_seen(buffers):
             assert buffers.in_place(a, b, *results)
 
 
+def test_instances_by_xcd_stay_within_the_first_axis(tmp_path):
+    "fewer than 2^32 work-items along x: an ensemble too large for that goes as (workgroups, instances)"
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    (tmp_path / "g.cpp").write_text('#include "lookup_grid.h"\nextern "C" int spread(size_t batch, size_t blocks) { return lk_spread(batch, blocks, 0, 1); }\n')
+    subprocess.run(["g++", "-std=c++17", "-Wall", "-Werror", "-shared", "-fPIC", "-I", os.path.join(root, "tramp_amd", "csrc"),
+                    str(tmp_path / "g.cpp"), "-o", str(tmp_path / "g.so")], check=True)
+    lib = C.CDLL(str(tmp_path / "g.so"))
+    lib.spread.argtypes = [C.c_size_t] * 2
+    for batch in (7, 8, 64, 1024, 65528, 65535):
+        rounded = (batch + 7) // 8 * 8
+        most = (2**32 // 256 - 1) // rounded
+        assert rounded * most * 256 < 2**32 <= rounded * (most + 1) * 256
+        assert lib.spread(batch, most) and lib.spread(batch, 1) and not lib.spread(batch, most + 1) and not lib.spread(batch, 2**31)
+    assert not lib.spread(1, 1) and not lib.spread(9, 1)
+
+
 def test_iterate_refuses_bad_steps():
     ep = object.__new__(T.ExpectationPropagation)
     ep.default_stopping = T.EarlyStoppingEP()

@@ -20,6 +20,7 @@
 // passes are bound by memory (a few operations per element), the conversions are free next to the loads.
 #include "common.h"
 #include "lookup_buffers.h"
+#include "lookup_grid.h"
 #include "tramp_math.h"
 
 #include <algorithm>
@@ -1076,13 +1077,6 @@ extern "C" int tramp_lookup_destroy(tramp_ctx* ctx, tramp_lookup* lk) {
         default: CALL(LK_LINES);          \
     }
 
-// Instances by XCD (lk_place): for what is read out of order in elements or rows, while it stays in an L2 of 4 MiB - the table of
-// an instance for a lookup or a message by position (up to twice that: 8 x 20000 x 64 f32 18.2 -> 14.3 us; 64 x 200000 f64 82 ->
-// 53 us), its positions for the sums (64 x 100000 f64, gradient 102 -> 92 us; 8 x 17 MB would be 169 -> 178 us) - and while the
-// last round of eight leaves few XCDs idle.
-static int lk_spread(size_t batch, size_t blocks, size_t bytes, size_t most) {
-    return batch > 1 && bytes <= most && (batch + 7) / 8 * 8 * 7 <= batch * 8 && (batch + 7) / 8 * 8 * blocks < 0x7fffffffu;
-}
 static dim3 lk_grid(size_t batch, size_t blocks, int spread) {
     return spread ? dim3((unsigned)((batch + 7) / 8 * 8 * blocks)) : dim3((unsigned)blocks, (unsigned)batch);
 }
@@ -1097,7 +1091,7 @@ static int lookup_apply(tramp_ctx* ctx, const tramp_lookup* lk, size_t batch, co
                            (unsigned)nb, (unsigned)batch, spread, lk->tok, z, x);
     } else {
         const size_t per = (size_t)4 * (kBlock >> lk->lw), nb = (lk->T + per - 1) / per;
-        TRAMP_REQUIRE(ctx, nb * lk->tiles < 0x7fffffffu);
+        TRAMP_REQUIRE(ctx, nb * lk->tiles <= kLkMaxGrid);
         const int spread = lk_spread(batch, nb * lk->tiles, lk->V * lk->D * sizeof(T), 8u << 20);
         const dim3 grid = lk_grid(batch, nb * lk->tiles, spread);
 #define LK_CALL(ROW)                                                                                                                   \
@@ -1200,8 +1194,7 @@ static int launch_rows(tramp_ctx* ctx, const tramp_lookup* lk, size_t batch, con
     a.pad0 = lk->seen;
     a.single_blocks = (unsigned)(((size_t)a.n_single + a.n_pad + kOne * G - 1) / (kOne * G));
     const size_t blocks = (size_t)a.n_lead + a.n_joins + a.n_runs + a.wave_blocks + a.light_blocks + a.single_blocks + (a.n_empty + kEmpty * G - 1) / (kEmpty * G);
-    TRAMP_REQUIRE(ctx, blocks * lk->tiles < 0x7fffffffu && (size_t)lk->n_spreads * lk->tiles < 0x7fffffffu &&
-                           (size_t)lk->n_chunks * lk->tiles < 0x7ffffffeu);
+    TRAMP_REQUIRE(ctx, blocks * lk->tiles <= kLkMaxGrid && (size_t)lk->n_chunks * lk->tiles < kLkMaxGrid);   // (as many spreads as chunks)
     a.blocks = (unsigned)blocks;
     a.spread = lk_spread(batch, blocks * lk->tiles, lk->T * lk->D * sizeof(T), 2u << 20);
     // few workgroups and few counts: each makes the scalars for itself, one launch less (V = 1000, 2000 positions 10.2 -> 7.6 us;
