@@ -1579,7 +1579,7 @@ class LookupChannel(Channel):
         return self._linear("tramp_lookup_apply", z, False, out)
 
     def gradient(self, x, out=None):
-        "the adjoint: row v is scale times the sum of x over the positions of token v, added in the order of the positions"
+        "the adjoint: row v is scale times the sum of x over the positions of token v, in an order fixed by the tokens alone"
         return self._linear("tramp_lookup_gradient", x, True, out)
 
     def sample(self, Z):

@@ -48,7 +48,7 @@ struct tramp_lookup {
     const LkItem* spreads;       // the chunks' positions
     const LkItem* runs;          // runs for one workgroup
     const LkItem* waves;         // runs for one wave
-    const LkItem* light;         // the shorter runs, by falling length; slot: the first position
+    const LkItem* light;         // the shorter runs, by falling length; slot: the first position, which the runs of one are read by
     const int* empty;            // rows without positions
     const int* idx;              // [V] place among the runs of two and more positions (short rows only)
     const int* code;             // [T] that place, -1 where padded, -2 - token where the run is this position (short rows only)
@@ -338,9 +338,9 @@ struct LkArgs {
 enum { LK_GRAD = 0, LK_BWD = 1, LK_FWD = 2, LK_MEAN = 3, LK_LOGZ = 4 };
 
 // rows perm[j0 + sub], perm[j0 + sub + S], ... of the run [j0, j0 + c), S = 1 << ls: added into acc, C in flight; KEEP: there are
-// at most C and they stay in `rows`.  p0: the position of a run of one, if known.
+// at most C and they stay in `rows`.
 template <typename T, int ROW, int C, bool KEEP, bool ONCE>
-__device__ __forceinline__ void lk_gather(const LkArgs& a, const T* __restrict__ xb, const LkLane& k, int j0, int c, int sub, int ls, int p0,
+__device__ __forceinline__ void lk_gather(const LkArgs& a, const T* __restrict__ xb, const LkLane& k, int j0, int c, int sub, int ls,
                                           double (&acc)[LkVec<T>::N], int (&pj)[C], T (&rows)[C][LkVec<T>::N]) {
     constexpr int N = LkVec<T>::N, Q = C < 4 ? C : 4;
     const int cnt = c > sub ? ((c - sub - 1) >> ls) + 1 : 0;
@@ -350,7 +350,7 @@ __device__ __forceinline__ void lk_gather(const LkArgs& a, const T* __restrict__
         for (int q = 0; q < C; q += Q)
             if (base + q < cnt) {
 #pragma unroll
-                for (int i = q; i < q + Q; ++i) pj[i] = i == 0 && c == 1 && p0 >= 0 ? p0 : base + i < cnt ? pp[(size_t)(base + i) << ls] : -1;
+                for (int i = q; i < q + Q; ++i) pj[i] = base + i < cnt ? pp[(size_t)(base + i) << ls] : -1;
             }
 #pragma unroll
         for (int q = 0; q < C; q += Q)
@@ -473,7 +473,7 @@ __device__ __forceinline__ void lk_chunk(const LkArgs& a, const LkLane& k, size_
     T rows[kKeep][N];
 #pragma unroll
     for (int e = 0; e < N; ++e) acc[e] = 0.0;
-    if (k.valid > 0) lk_gather<T, ROW, kKeep, false, ONCE>(a, xb, k, it.start, it.end - it.start, k.group, 8 - a.lw, -1, acc, pj, rows);
+    if (k.valid > 0) lk_gather<T, ROW, kKeep, false, ONCE>(a, xb, k, it.start, it.end - it.start, k.group, 8 - a.lw, acc, pj, rows);
     lk_block_join<N>(k, acc, sm);
     if (threadIdx.x >= (1u << a.lw) || k.valid <= 0) return;
     double* p = partials + (b * a.n_chunks + (size_t)it.slot) * a.D + k.col;
@@ -532,7 +532,7 @@ __global__ __launch_bounds__(kBlock) void lookup_rows_kernel(LkArgs a, LkScalArg
     T rows[kKeep][N], z[N];
 #pragma unroll
     for (int e = 0; e < N; ++e) acc[e] = 0.0;
-    int v, j0, count, sub, ls, p0 = -1, place_ws = -1;
+    int v, j0, count, sub, ls, place_ws = -1;
     bool first = true;
     // the row of the table is asked for as soon as it is known, the sum comes later
     const auto row_of = [&](int v) {
@@ -563,7 +563,7 @@ __global__ __launch_bounds__(kBlock) void lookup_rows_kernel(LkArgs a, LkScalArg
         sub = k.group;
         ls = 8 - a.lw;
         first = threadIdx.x < (1u << a.lw);
-        if (act) lk_gather<T, ROW, kKeep, MODE == LK_FWD && !LONG, true>(a, xb, k, j0, count, sub, ls, p0, acc, pj, rows);
+        if (act) lk_gather<T, ROW, kKeep, MODE == LK_FWD && !LONG, true>(a, xb, k, j0, count, sub, ls, acc, pj, rows);
         lk_block_join<N>(k, acc, sm);
     } else {
         blk -= a.n_runs;
@@ -643,7 +643,6 @@ __global__ __launch_bounds__(kBlock) void lookup_rows_kernel(LkArgs a, LkScalArg
                 row_of(v);
                 j0 = it.start;
                 count = it.end - it.start;
-                p0 = it.slot;
             } else {
                 v = (int)u;
                 row_of(v);
@@ -662,7 +661,7 @@ __global__ __launch_bounds__(kBlock) void lookup_rows_kernel(LkArgs a, LkScalArg
                 constexpr int C = decltype(depth)::value;
                 int qj[C];
                 T part[C][N];
-                lk_gather<T, ROW, C, true, true>(a, xb, k, j0, count, 0, 0, p0, acc, qj, part);
+                lk_gather<T, ROW, C, true, true>(a, xb, k, j0, count, 0, 0, acc, qj, part);
                 if (MODE == LK_GRAD || MODE == LK_BWD) {
                     lk_row_out<T, ROW, MODE>(a, c, k, b, v, count, acc, z, damping, b_old, out, r_out);
                     return;
@@ -686,13 +685,13 @@ __global__ __launch_bounds__(kBlock) void lookup_rows_kernel(LkArgs a, LkScalArg
             if (!act) return;
             if (four)
                 run(std::integral_constant<int, 4>{});
-            else if (two)
+            else if (MODE == LK_FWD || MODE == LK_MEAN || two)     // these come from the list of runs of two and more
                 run(std::integral_constant<int, 2>{});
             else
                 run(std::integral_constant<int, 1>{});
             return;
         }
-        if (act) lk_gather<T, ROW, kKeep, true, true>(a, xb, k, j0, count, sub, ls, p0, acc, pj, rows);
+        if (act) lk_gather<T, ROW, kKeep, true, true>(a, xb, k, j0, count, sub, ls, acc, pj, rows);
         if (ls) lk_wave_join<N>(a.lw, acc);
     }
     if (MODE == LK_LOGZ) {
@@ -876,7 +875,7 @@ __global__ __launch_bounds__(kBlock) void lookup_positions1_kernel(LkArgs a, con
 
 // ---------------------------------------------------------------- log-partition
 // A = 1/2 sum_v (bz + g)^2 / prec + D/2 sum_v log(2 pi / prec)   (linear_channel.py:127-132): the rows' shares, one double per row
-// and column tile, added in two steps.  Once per run, not per iteration; bound like the message to the table.
+// and column tile, added in two steps.  At the end of a run, but for every candidate of every edge under adaptive damping.
 __global__ __launch_bounds__(kBlock) void lookup_fold_kernel(size_t n, const double* __restrict__ in, double* __restrict__ out) {
     __shared__ double smem[kBlock / kWave];
     const size_t b = blockIdx.y;
