@@ -275,9 +275,9 @@ TM_HD float erfcx_tay(float x) {
     }
     return acc;
 }
-// Two f32 evaluations at once on the packed-f32 pipe (v_pk_fma_f32 / v_pk_mul_f32 / v_pk_add_f32: two lanes' worth per
-// issue; plain f32 issues at the f64 rate on gfx950, which is what bounds the f32 two-region channels): the two regions of
-// a K7 component are the pair.  Same operations in the same order as erfcx_tay(float): bit-identical results.
+// Two f32 evaluations at once: the two components of a call of OpPair's ops (ew_ops.h).  The library is compiled without packed f32
+// instructions, so a two-element operation is two plain ones; what a pair brings is two chains of dependent instructions side by
+// side (times at OpPair).  Same operations in the same order as erfcx_tay(float): bit-identical results.
 typedef float tm_v2f __attribute__((ext_vector_type(2)));
 #if defined(__HIPCC__)
 __device__ __forceinline__ tm_v2f erfcx_tay_v2(tm_v2f x) {
@@ -654,7 +654,7 @@ template <typename T> TM_HD RV<T> sgn_lik_posterior_lean(T bz, T y, const Region
 }
 
 #if defined(__HIPCC__) && TRAMP_ERFCX_UNIFORM
-// Two f32 components at once on the packed-f32 pipe (erfcx_tay_v2): the same operations in the same order as the scalar form.
+// Two f32 components at once (erfcx_tay_v2): the same operations in the same order as the scalar form.
 __device__ __forceinline__ void sgn_lik_posterior_lean_v2(tm_v2f bz, tm_v2f y, const RegionConst<float>& c, tm_v2f* r, tm_v2f* v, tm_v2f* dev) {
     const tm_v2f r0 = (bz * y) * c.v0;
     const tm_v2f x = ((0.0f - r0) * c.inv_s0) * 0.70710678118654752440f;
@@ -1099,10 +1099,10 @@ TM_HD bool pwl_moment_form(T bz, T bx, const PwlConst<T>& c, PwlOut<T>& o, T* de
 }
 
 #if defined(__HIPCC__) && TRAMP_ERFCX_UNIFORM
-// The lean moment form (VOTE = false, the uniform-grid erfcx table) for TWO f32 components at once on the packed-f32 pipe:
-// the lanes of every two-lane operation are the two components, so there is no horizontal sum and no cross-lane select -
-// the same operations in the same order as pwl_moment_form<float, ..., false> per lane.  (Plain f32 issues at the f64
-// rate on gfx950; the f32 K7 updates are instruction-bound at half f64's bytes.)
+// The lean moment form (VOTE = false, the uniform-grid erfcx table) for TWO f32 components at once: the elements of every
+// two-element operation are the two components, so there is no horizontal sum and no select between them - the same operations in
+// the same order as pwl_moment_form<float, ..., false> per element.  (Plain f32 issues at the f64 rate on gfx950; the f32 K7
+// updates are instruction-bound at half f64's bytes.)
 __device__ __forceinline__ tm_v2f v2_min(tm_v2f a, tm_v2f b) { return tm_v2f{fmin_(a.x, b.x), fmin_(a.y, b.y)}; }
 __device__ __forceinline__ tm_v2f v2_max(tm_v2f a, tm_v2f b) { return tm_v2f{fmax_(a.x, b.x), fmax_(a.y, b.y)}; }
 __device__ __forceinline__ tm_v2f v2_sel(bool cx, bool cy, tm_v2f a, tm_v2f b) { return tm_v2f{cx ? a.x : b.x, cy ? a.y : b.y}; }
