@@ -588,7 +588,8 @@ int tramp_lookup_log_partition(tramp_ctx* ctx, tramp_lookup* lookup, size_t batc
 
 /* ---- lists of arrays: global norm, clipping, bounded steps -------------------------- */
 /* k arrays [batch, n_i] of one element type; row b of all of them is instance b, whose global norm is
- * |x_b| = sqrt(sum over the arrays and components of x^2), summed in double in a fixed order.  arrays_d: host array of device
+ * |x_b| = sqrt(sum over the arrays and components of x^2), summed in double in a fixed order (f64 components beyond 1e154
+ * make it infinite, the squares of those below 1e-162 are 0).  arrays_d: host array of device
  * pointers, kept as they are (the caller keeps the arrays alive and in place); the arrays must not overlap. */
 typedef struct tramp_group tramp_group;
 int tramp_group_create(tramp_ctx* ctx, int dtype, int k, void* const* arrays_d, const size_t* n, size_t batch, tramp_group** group);

@@ -415,3 +415,26 @@ def test_a_step_that_is_not_finite_reaches_the_guard(ctx):
                                    @ T.SISOVariable(id="z") @ T.GaussianLikelihood(y=y, var=0.1, ctx=ctx)).to_model(), ctx=ctx)
     with pytest.raises(ValueError, match="nan"):
         ep.iterate(max_iter=5, max_step=1.0)
+
+
+@pytest.mark.parametrize("seed", range(3))
+def test_uneven_counts_damped_and_bounded(ctx, seed):
+    """A categorical regression that undamped sweeps do not solve: constant damping and a bounded step both meet the stopping rule, at
+    one fixed point.  A run whose change falls below 1e-6 in at most 200 sweeps contracts by 1e-6 ** (1 / 200) = 0.933 a sweep or
+    better, so it is within 1e-6 / (1 - 0.933) = 1.5e-5 of its fixed point; 1e-4 holds two of them."""
+    import tramp_amd as T
+    rs = np.random.RandomState(seed)
+    V, n = 1000, 2000
+    tok = zipf_tokens(rs, V, n, 1.0)
+    x = orc.gb_sample(rs, V, 0.5)
+    y = x[tok] + np.sqrt(0.1) * rs.standard_normal(n)
+    r, sweeps = [], []
+    for kw in (dict(damping=0.3), dict(max_step=10.0)):
+        model = (T.GaussBernoulliPrior(size=V, rho=0.5, ctx=ctx) @ T.SISOVariable(id="x") @ T.LookupChannel(tok, V, ctx=ctx)
+                 @ T.SISOVariable(id="z") @ T.GaussianLikelihood(y=y, var=0.1, ctx=ctx)).to_model()
+        ep = T.ExpectationPropagation(model, ctx=ctx).iterate(max_iter=200, callback=T.EarlyStoppingEP(tol=1e-6, max_increase=np.inf), **kw)
+        assert ep.status[0] == 1, kw
+        r.append(ep.get_variables_data()["x"]["r"].reshape(-1))
+        sweeps.append(int(ep.n_iter_instance[0]))
+    assert sweeps[0] < sweeps[1]                                       # the bound is the slower of the two
+    assert np.linalg.norm(r[0] - r[1]) < 1e-4 * np.linalg.norm(r[0])

@@ -1182,8 +1182,10 @@ class ExpectationPropagation:
         is raised (message_passing.py:187-209, callbacks.py:233-240,277-283); a warm start then continues each
         instance from where its own run would have stopped.
         ``max_step`` bounds the step of an iteration: the norm of new minus old b over all messages of an instance; a
-        longer step is shortened to it, precisions included, on top of constant damping.  ``step_norm`` holds the norms
-        before the bound, per instance (double[batch] on the device, of the last iteration)."""
+        longer step is shortened to it, precisions included, on top of constant damping.  It keeps a run finite whose
+        undamped messages blow up; constant damping, where it converges, takes fewer iterations and is the one to try
+        first.  ``step_norm`` holds the norms before the bound, per instance (double[batch] on the device, of the last
+        iteration)."""
         if update_dA:
             raise NotImplementedError("update_dA (the per-message free-energy increments of message_passing.py:245-246) is not tracked")
         initializer = initializer or ConstantInit(a=0, b=0)

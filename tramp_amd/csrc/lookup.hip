@@ -503,7 +503,8 @@ __global__ __launch_bounds__(kBlock) void lookup_chunks_kernel(LkArgs a, LkScalA
 // Bound by the bytes where a row fills its lines: the other 378000 positions of that message, 207 MB read and written, 47 us,
 // 4.4 TB/s; gradient of 65536 x 1024 f32 to 32000 rows 246 MB 46 us, 5.3 TB/s, after 23 us for 110 MB of heavy runs.  Rows that
 // share lines are bound by the lines: 168 bytes touch 2.3 of 128 on average, message of 8 x 80021 x 21 f64 to 10007 rows 34 us;
-// one column by a line from the L2 per element, 8 bytes of 128: gradient of 1000001 f64 17 us.
+// one column by lines fetched again: every XCD gathers from all of x, more than its L2 of 4 MiB holds, and the 8 MB of 1000001 f64
+// come past the L2s eleven times, 88 MB in 17 us.
 template <typename T, int ROW, int MODE, bool SELF, bool LONG>
 __global__ __launch_bounds__(kBlock) void lookup_rows_kernel(LkArgs a, LkScalArgs q, const LkScal* __restrict__ scal, const T* __restrict__ bz,
                                                              const T* __restrict__ x, double damping, const T* b_old, T* out,
@@ -782,9 +783,10 @@ __global__ __launch_bounds__(kBlock) void lookup_spread_kernel(LkArgs a, const L
 // Rows shorter than half a line cost a line each when they are read or written in the order of the tokens.  Here the sums of the
 // runs of two and more positions leave scale r in double (LK_MEAN), and x is walked in its own order: a position that is
 // alone in its run has its sum at hand, the others fetch theirs.  One column: a lane takes one 16-byte piece of positions.  Bound
-// by the lines a gather takes from the L2: 64 instances of 100000 positions of 200000 f64, 6.4 10^6 gathers, 44 us, and 37 us for
-// the sums before.  Dropped: runs of two and three summed at each of their positions (102 us in all against 99), two pieces per lane
-// (100).
+// by memory: 64 instances of 100000 positions of 200000 f64 take 44 us, after 37 us for the sums, and the two launches miss the L2
+// on 3.1 10^6 lines, 400 MB where z, x and the result are 205 MB: all instances pass the first launch before one passes the second,
+// which finds nothing of its own in an L2.  Dropped: runs of two and three summed at each of their positions (102 us in all against
+// 99), two pieces per lane (100).
 template <typename T, int ROW>
 __global__ __launch_bounds__(kBlock) void lookup_positions_kernel(LkArgs a, const int* __restrict__ code, const LkScal* __restrict__ scal,
                                                                   const T* __restrict__ bz, const double* __restrict__ sr_ws,
@@ -876,6 +878,8 @@ __global__ __launch_bounds__(kBlock) void lookup_positions1_kernel(LkArgs a, con
 // ---------------------------------------------------------------- log-partition
 // A = 1/2 sum_v (bz + g)^2 / prec + D/2 sum_v log(2 pi / prec)   (linear_channel.py:127-132): the rows' shares, one double per row
 // and column tile, added in two steps.  At the end of a run, but for every candidate of every edge under adaptive damping.
+// Rows that nobody reads, or one position, have no kind of their own here: 8 x 10007 x 21 f64 of 80021 positions 48 us (the message to
+// the table 39), 64 x 200000 f64 of 100000 146 us (98), 50000 x 64 f32 of 10^6 63 us (56).
 __global__ __launch_bounds__(kBlock) void lookup_fold_kernel(size_t n, const double* __restrict__ in, double* __restrict__ out) {
     __shared__ double smem[kBlock / kWave];
     const size_t b = blockIdx.y;
